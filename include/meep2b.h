@@ -368,6 +368,135 @@ int meep2b_merge_stack(const void* weight, int32_t weight_dtype, const float* sc
                        const float* rhs, int32_t rank, float scaling, int64_t experts, int64_t rows, int64_t cols,
                        void* out, int32_t out_dtype, void* stream);
 
+/* ------------------------------------------------------------------------------------------------ vocabulary loss */
+
+enum meep2b_reduction { MEEP2B_REDUCE_NONE = 0, MEEP2B_REDUCE_MEAN = 1, MEEP2B_REDUCE_SUM = 2 };
+
+/* Softmax cross entropy of hidden states against a vocabulary's rows, l_tv = <h_t, W_v>, without the logits, and its
+ * gradients. hidden (tokens, hidden_size) and weight (vocab, hidden_size) in bf16, rows ld_* elements apart
+ * (multiples of 8, as is hidden_size; 16-byte aligned); targets (tokens) int64, `ignore_index` where there is none:
+ * such a token's loss and gradient are zero and nothing of its row is read. A target outside the vocabulary makes its
+ * token's loss and gradient NaN. The mean is over the tokens with a target (zero where there are none). At most 2^24
+ * tokens and 2^24 vocabulary rows. Sizes of the buffers come from meep2b_linear_ce_plan. */
+typedef struct meep2b_linear_ce {
+  const void* hidden;
+  int64_t tokens;
+  int64_t hidden_size;
+  int64_t ld_hidden;
+  const void* weight;
+  int64_t vocab;
+  int64_t ld_weight;
+  const int64_t* targets;
+  int64_t ignore_index;
+  int32_t reduction;       /* enum meep2b_reduction */
+  int32_t planes;          /* of acc */
+  int64_t rows_pad;        /* tokens up to a multiple of 256 */
+  int64_t piece_cols;      /* columns of a vocabulary piece, a multiple of 256; 0 with piece == NULL: one piece */
+  /* written by the forward pass, read by the backward pass */
+  int32_t* state;          /* 8 */
+  int32_t* flags;          /* rows_pad / 256 */
+  int32_t* source;         /* rows_pad: token of each live row */
+  int32_t* slot;           /* tokens: live row of each token, or -1 */
+  int32_t* target;         /* rows_pad */
+  float* row_values;       /* 5 * rows_pad */
+  void* compact;           /* (rows_pad, hidden_size) bf16: the live rows (backward: only with d_weight) */
+  float* acc;              /* planes * (rows_pad, hidden_size): the hidden states' gradient before its upstream scale;
+                              forward: NULL for the loss alone */
+  /* workspaces of one call */
+  void* piece;             /* (rows_pad, piece_cols) bf16; needed with acc (forward) and with d_weight (backward) */
+  float* part;             /* 2 * ceil(vocab / 256) * rows_pad (forward) */
+  float* row_loss;         /* rows_pad (forward, mean and sum) */
+  /* forward: tokens values (none) or one */
+  float* loss;
+  /* backward: the loss's gradient (tokens values or one), and what is asked for, contiguous */
+  const float* upstream;
+  void* d_hidden;          /* (tokens, hidden_size) bf16, or NULL */
+  void* d_weight;          /* (vocab, hidden_size) bf16, or NULL: the frozen head. With it the gradients are computed
+                              by the backward call (acc is then its workspace), else dh's planes by the forward call */
+} meep2b_linear_ce;
+
+/* rows_pad, piece_cols and planes for these sizes: a piece's buffer is at most 1 GB (or 256 columns), the planes
+ * 512 MB (or one). */
+int meep2b_linear_ce_plan(int64_t tokens, int64_t hidden_size, int64_t vocab, int64_t* rows_pad, int64_t* piece_cols,
+                          int32_t* planes);
+int meep2b_linear_ce_forward(const meep2b_linear_ce* a, void* stream);
+int meep2b_linear_ce_backward(const meep2b_linear_ce* a, void* stream);
+
+/* ------------------------------------------------------------------------------------------------ router balance */
+
+/* The load-balancing loss of Transformers' MoE models (load_balancing_loss_func) over the unmasked tokens of all
+ * layers, N of them: with p the float32 softmax of a token's logits, f_e the tokens (of N) that chose expert e over N and
+ * m_e the mean of p_e, loss = experts * sum_e f_e m_e, and its gradient of the logits (the choice carries none). The
+ * choice is `index` (tokens, top_k) per layer, or the top_k largest logits, the lower expert first where they are
+ * equal. logits: per layer (tokens, experts) contiguous, bf16 or f32. A masked token (mask byte 0) is not read; its
+ * gradient is zero. At most 128 layers and 1024 experts. */
+typedef struct meep2b_balance {
+  const void* const* logits;    /* host array of `layers` device pointers */
+  int32_t layers;
+  int32_t experts;
+  int64_t tokens;
+  int32_t top_k;
+  int32_t dtype;
+  const uint8_t* mask;          /* (tokens), or NULL */
+  const int64_t* const* index;  /* host array of device pointers, or NULL: choose here */
+  int64_t* counts;              /* forward, out: (layers, experts) tokens of each expert */
+  float* loss;                  /* forward, out */
+  float* coef;                  /* (experts): written by the forward pass, read by the backward pass */
+  void* workspace;              /* forward: meep2b_balance_workspace_bytes(experts) */
+  const float* upstream;        /* backward: the loss's gradient */
+  void* const* grads;           /* backward, out: host array of device pointers, as logits */
+} meep2b_balance;
+
+size_t meep2b_balance_workspace_bytes(int32_t experts);
+int meep2b_balance_loss(const meep2b_balance* a, void* stream);
+int meep2b_balance_loss_backward(const meep2b_balance* a, void* stream);
+
+/* ------------------------------------------------------------------------------------------------ head norms */
+
+/* RMS norm of every query and key head (its own weight for queries and for keys) and the rotation by position in one
+ * pass: y = R(pos) (x / sqrt(mean(x^2) + eps) * w). The first 2 half dimensions turn in pairs (i, i + half) by the
+ * angles whose cosines and sines are row pos of cos and sin (angles rows, ld_* elements apart, f32 or bf16); the others
+ * stay. q (batch, length, q_heads, dim) and k (batch, length, kv_heads, dim) in bf16 or f32 with unit inner stride;
+ * strides of the batch, the token and the head in elements, multiples of 16 bytes. positions (batch, length) int64, or
+ * NULL for 0 .. length - 1 in every batch; a position outside the angles makes its turned values NaN. dim a multiple of
+ * 16 up to 256, half of 8. Outputs are contiguous. */
+typedef struct meep2b_head_norm {
+  const void* q;
+  const void* k;
+  int64_t batch;
+  int64_t length;
+  int32_t q_heads;
+  int32_t kv_heads;
+  int32_t dim;
+  int32_t half;
+  int64_t q_stride[3];
+  int64_t k_stride[3];
+  int32_t dtype;
+  int32_t angle_dtype;
+  const void* q_weight;         /* (dim), as q */
+  const void* k_weight;
+  const void* cos;
+  const void* sin;
+  int64_t ld_cos;
+  int64_t ld_sin;
+  int64_t angles;
+  const int64_t* positions;
+  float eps;
+  void* q_out;                  /* forward: the outputs; backward: the gradients of q and k */
+  void* k_out;
+  const void* dq_out;           /* backward: the outputs' gradients */
+  const void* dk_out;
+  int64_t dq_out_stride[3];
+  int64_t dk_out_stride[3];
+  void* dq_weight;              /* backward: the weights' gradients, or both NULL */
+  void* dk_weight;
+  float* partial;               /* backward, with them: meep2b_head_norm_partials() * dim */
+} meep2b_head_norm;
+
+int meep2b_head_norm_partials(void);
+int meep2b_head_norm_rotate(const meep2b_head_norm* a, void* stream);
+int meep2b_head_norm_rotate_backward(const meep2b_head_norm* a, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -48,6 +48,42 @@ class ProductF8(ctypes.Structure):
     ]
 
 
+class LinearCE(ctypes.Structure):
+    """struct meep2b_linear_ce (include/meep2b.h)."""
+
+    _fields_ = [
+        ("hidden", _p), ("tokens", _i64), ("hidden_size", _i64), ("ld_hidden", _i64),
+        ("weight", _p), ("vocab", _i64), ("ld_weight", _i64), ("targets", _p), ("ignore_index", _i64),
+        ("reduction", _i32), ("planes", _i32), ("rows_pad", _i64), ("piece_cols", _i64),
+        ("state", _p), ("flags", _p), ("source", _p), ("slot", _p), ("target", _p), ("row_values", _p),
+        ("compact", _p), ("acc", _p), ("piece", _p), ("part", _p), ("row_loss", _p), ("loss", _p),
+        ("upstream", _p), ("d_hidden", _p), ("d_weight", _p),
+    ]
+
+
+class Balance(ctypes.Structure):
+    """struct meep2b_balance (include/meep2b.h)."""
+
+    _fields_ = [
+        ("logits", _p), ("layers", _i32), ("experts", _i32), ("tokens", _i64), ("top_k", _i32), ("dtype", _i32),
+        ("mask", _p), ("index", _p), ("counts", _p), ("loss", _p), ("coef", _p), ("workspace", _p),
+        ("upstream", _p), ("grads", _p),
+    ]
+
+
+class HeadNorm(ctypes.Structure):
+    """struct meep2b_head_norm (include/meep2b.h)."""
+
+    _fields_ = [
+        ("q", _p), ("k", _p), ("batch", _i64), ("length", _i64), ("q_heads", _i32), ("kv_heads", _i32),
+        ("dim", _i32), ("half", _i32), ("q_stride", _i64 * 3), ("k_stride", _i64 * 3), ("dtype", _i32),
+        ("angle_dtype", _i32), ("q_weight", _p), ("k_weight", _p), ("cos", _p), ("sin", _p), ("ld_cos", _i64),
+        ("ld_sin", _i64), ("angles", _i64), ("positions", _p), ("eps", _f32), ("q_out", _p), ("k_out", _p),
+        ("dq_out", _p), ("dk_out", _p), ("dq_out_stride", _i64 * 3), ("dk_out_stride", _i64 * 3),
+        ("dq_weight", _p), ("dk_weight", _p), ("partial", _p),
+    ]
+
+
 _SIGNATURES = {
     "meep2b_version": (ctypes.c_char_p, []),
     "meep2b_status_string": (ctypes.c_char_p, [ctypes.c_int]),
@@ -84,6 +120,16 @@ _SIGNATURES = {
     "meep2b_grouped_product_f8": (ctypes.c_int, [ctypes.POINTER(ProductF8), _p]),
     "meep2b_swiglu": (ctypes.c_int, [_p, _i64, _i64, _p, _p]),
     "meep2b_swiglu_backward": (ctypes.c_int, [_p, _p, _i64, _i64, _p, _p]),
+    "meep2b_balance_workspace_bytes": (_sz, [_i32]),
+    "meep2b_balance_loss": (ctypes.c_int, [ctypes.POINTER(Balance), _p]),
+    "meep2b_balance_loss_backward": (ctypes.c_int, [ctypes.POINTER(Balance), _p]),
+    "meep2b_head_norm_partials": (ctypes.c_int, []),
+    "meep2b_head_norm_rotate": (ctypes.c_int, [ctypes.POINTER(HeadNorm), _p]),
+    "meep2b_head_norm_rotate_backward": (ctypes.c_int, [ctypes.POINTER(HeadNorm), _p]),
+    "meep2b_linear_ce_plan": (ctypes.c_int, [_i64, _i64, _i64, ctypes.POINTER(_i64), ctypes.POINTER(_i64),
+                                             ctypes.POINTER(_i32)]),
+    "meep2b_linear_ce_forward": (ctypes.c_int, [ctypes.POINTER(LinearCE), _p]),
+    "meep2b_linear_ce_backward": (ctypes.c_int, [ctypes.POINTER(LinearCE), _p]),
 }
 
 _lib = None
@@ -140,6 +186,10 @@ KERNELS_PER_CALL = {
     "meep2b_merge_stack": 1,
     "meep2b_quant_multipliers": 1, "meep2b_fp8_rows_quantize": 1, "meep2b_grouped_product_f8": 1,
     "meep2b_swiglu": 1, "meep2b_swiglu_backward": 1, "meep2b_weight_grad": 1, "meep2b_combine": 1,
+    "meep2b_balance_loss": 2, "meep2b_balance_loss_backward": 1,
+    # at least: one more per vocabulary piece and gradient, and with the weights' gradients
+    "meep2b_linear_ce_plan": 0, "meep2b_linear_ce_forward": 4, "meep2b_linear_ce_backward": 1,
+    "meep2b_head_norm_rotate": 1, "meep2b_head_norm_rotate_backward": 1,
 }
 launches = {}
 

@@ -1,0 +1,907 @@
+// The language-model loss of hidden states against a large vocabulary, without the logits: softmax cross entropy of
+// l_tv = <h_t, W_v> against one target per row, its gradient of the hidden states and of the head.
+//
+// With the target's own logit as each row's reference, q_tv = exp(l_tv - l_t,y) and Z_t = 1 + sum_{v != y} q_tv:
+//   loss_t  = log Z_t
+//   dh_t    = g_t ((sum_{v != y} q_tv W_v) / Z_t - (1 - 1/Z_t) W_y)
+//   dW_v    = sum_t g_t (q_tv / Z_t - [v = y_t]) h_t
+// The reference is known before the products (one dot product per row), so that a tile of q is final when it leaves
+// its accumulator: no running maximum, no rescaling of what was summed before, and dh needs one pass over the
+// vocabulary (the logits' product and the product with W), not a second one for the normaliser. bf16 has float32's
+// exponents, so q may lie anywhere within 2^+-96 of the target without losing bits. A 32-column piece of a row whose
+// sum leaves that window is summed against its own maximum instead (its logarithm is what is kept, as a negative
+// number), and the row tiles that hold such rows have their q and their dh product computed again with the row's
+// log-sum as the reference, by launches that return at once where there are none.
+//
+// Only rows with a target are computed: they are copied to the front of a buffer first (the scan and the gather
+// below), which also keeps what stands in ignored rows, infinities and NaN included, out of every sum.
+//
+// The products are one persistent tcgen05 kernel on CTA pairs (M = 256, N = 256, K = 64 a stage, both operands by
+// TMA, two accumulators in tensor memory), with a mode for each epilogue:
+//   kStats    the row sums of a 256-column tile (two 128-column halves), nothing else
+//   kProbs    the same, and q as bf16 into the vocabulary piece's buffer
+//   kReprobs  q alone, for the row tiles to be computed again
+//   kGrad     g (q / Z - [v = y]) as bf16 into the piece's buffer (the head's gradient, and dh beside it)
+//   kAcc      dh's product: piece x W, float32, stored by the first piece and added (TMA reduction) by the others
+//   kWeight   dW's product: piece^T x h, bf16
+#include "common.cuh"
+#include "host.hpp"
+
+namespace meep2b {
+namespace vocab {
+
+constexpr int TILE = 256;   // rows and columns of a unit (a CTA pair)
+constexpr int BK = 64;
+constexpr int STAGES = 6;
+constexpr int OPERAND_BYTES = 128 * BK * 2;  // each CTA's half of A or of B, one stage
+constexpr int STAGE_BYTES = 2 * OPERAND_BYTES;
+constexpr int THREADS = 384;
+constexpr int EPI_WARP0 = 4;
+constexpr int STG_BYTES = 4096;  // per epilogue warp
+constexpr int OFF_STG = STAGES * STAGE_BYTES;
+constexpr int OFF_BAR = OFF_STG + 8 * STG_BYTES;
+constexpr int NUM_BARS = 2 * STAGES + 5;
+constexpr int OFF_TMEM = OFF_BAR + NUM_BARS * 8;
+constexpr int SMEM_BYTES = OFF_TMEM + 16 + 1024;
+constexpr uint32_t TMEM_COLS = 512;
+constexpr int GROUP = 8;  // row tiles that share a column tile before the next column tile is taken
+static_assert(SMEM_BYTES <= 232448, "shared memory plan exceeds 227 KB");
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kWindow = 7.9228162514264338e28f;  // 2^96
+
+enum Mode { kStats, kProbs, kReprobs, kGrad, kAcc, kWeight };
+
+// ints of `state`
+enum { kLive = 0, kRedo = 1, kDone = 2, kStateInts = 8 };
+
+struct Rows {  // per live row, float32
+  float* ref;    // the reference of q, in units of log 2 (after a recomputation: the row's log-sum)
+  float* logit;  // the target's logit
+  float* lse;    // log2 of the sum of 2^(logit / log 2) over the vocabulary
+  float* scale;  // what q is multiplied by to be the probability: 2^(ref - lse)
+  float* miss;   // 1 - the target's probability
+};
+
+struct Params {
+  const int32_t* state;
+  const int32_t* flags;    // row tiles to compute again
+  const int32_t* target;   // per live row (-1 past the last)
+  const int32_t* source;   // the live row's token
+  Rows rows;
+  float* part;             // (2 * column tiles of the vocabulary) x rows_pad: the row sums
+  int64_t rows_pad;
+  const float* upstream;   // one value, or one per token
+  int per_token, mean;     // how g follows from it
+  int vocab, hidden;
+  int v0, piece_tiles;     // the piece: its first column and its column tiles
+  int k_total;             // depth of the product, in elements (kAcc: the piece's columns; kWeight: live rows)
+  int planes;              // kAcc: the most parts the depth may be split into, each summed in a plane of its own
+  int first;               // kAcc: the first piece (stores)
+};
+
+// Into how many parts the depth of a product of `units` tiles is split on `pairs` CTA pairs: the number whose last
+// round of units leaves the least idle, each part costing about 1% of a round (its plane written and read again).
+__host__ __device__ inline int depth_parts(int units, int pairs, int most) {
+  int best = 1;
+  float best_cost = 1e30f;
+  for (int s = 1; s <= most; ++s) {
+    const float cost = static_cast<float>((units * s + pairs - 1) / pairs) / s + 0.01f * s;
+    if (cost < best_cost) best_cost = cost, best = s;
+  }
+  return best;
+}
+
+struct Units {
+  int mt, nt, parts, total, kblocks;
+
+  __device__ void decode(int u, int& m, int& n, int& part) const {
+    const int per = mt * nt;
+    part = u / per;
+    int r = u - part * per;
+    const int group = r / (GROUP * nt);
+    const int rows = min(GROUP, mt - group * GROUP);
+    r -= group * GROUP * nt;
+    n = r / rows;
+    m = group * GROUP + (r - n * rows);
+  }
+  __device__ int k_begin(int part) const { return static_cast<int>(static_cast<int64_t>(kblocks) * part / parts); }
+};
+
+template <int MODE>
+__device__ __forceinline__ Units units_of(const Params& p, int pairs) {
+  Units w;
+  const int live = p.state[kLive];
+  const int row_tiles = (live + TILE - 1) / TILE;
+  if (MODE == kWeight) {
+    w.mt = p.piece_tiles, w.nt = (p.hidden + TILE - 1) / TILE, w.parts = 1;
+    w.kblocks = (live + BK - 1) / BK;
+  } else if (MODE == kAcc) {
+    w.mt = row_tiles, w.nt = (p.hidden + TILE - 1) / TILE;
+    w.parts = depth_parts(w.mt * w.nt, pairs, p.planes);
+    w.kblocks = (p.k_total + BK - 1) / BK;
+  } else {
+    w.mt = row_tiles, w.nt = p.piece_tiles, w.parts = 1;
+    w.kblocks = (p.hidden + BK - 1) / BK;
+  }
+  w.total = w.mt * w.nt * w.parts;
+  return w;
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ void tma_add_2d(const CUtensorMap* map, uint32_t src, int32_t c0, int32_t c1) {
+  asm volatile("cp.reduce.async.bulk.tensor.2d.global.shared::cta.add.tile.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(src), "r"(c0), "r"(c1)
+               : "memory");
+}
+
+// The row `lane` of a tile of 32 rows x 32 bf16 (64-byte swizzle), or of 32 rows x 32 float32 (128-byte swizzle).
+__device__ __forceinline__ void stage_bf16(uint32_t tile, int lane, const uint32_t (&w)[16]) {
+  const uint32_t r = tile + static_cast<uint32_t>(lane) * 64u;
+  const uint32_t sw = (static_cast<uint32_t>(lane) >> 1) & 3u;
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(r + ((static_cast<uint32_t>(j) ^ sw) << 4)),
+                 "r"(w[4 * j]), "r"(w[4 * j + 1]), "r"(w[4 * j + 2]), "r"(w[4 * j + 3])
+                 : "memory");
+}
+
+__device__ __forceinline__ void stage_f32(uint32_t tile, int lane, const float (&v)[32]) {
+  const uint32_t r = tile + static_cast<uint32_t>(lane) * 128u;
+  const uint32_t sw = static_cast<uint32_t>(lane) & 7u;
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(r + ((static_cast<uint32_t>(j) ^ sw) << 4)),
+                 "r"(__float_as_uint(v[4 * j])), "r"(__float_as_uint(v[4 * j + 1])),
+                 "r"(__float_as_uint(v[4 * j + 2])), "r"(__float_as_uint(v[4 * j + 3]))
+                 : "memory");
+}
+
+// g of a live row: the loss's upstream gradient over the reduction.
+__device__ __forceinline__ float row_upstream(const float* upstream, int per_token, int mean, int token, int live) {
+  const float g = upstream[per_token ? token : 0];
+  return mean ? g / static_cast<float>(max(live, 1)) : g;
+}
+
+// One unit's epilogue for one warp: 32 rows (a lane each) and 128 columns, 32 at a time.
+template <int MODE>
+__device__ __forceinline__ void epilogue(const Params& p, const CUtensorMap* out, int m, int n, int part, bool empty,
+                                         int row0, int half, uint32_t acc, int lane, uint32_t stg, uint32_t tempty,
+                                         int live) {
+  const int row = row0 + lane;  // of the live rows (kWeight: of the piece's columns)
+  constexpr bool LOGITS = MODE == kStats || MODE == kProbs || MODE == kReprobs || MODE == kGrad;
+  const int c_first = n * TILE + half * 128;  // column of the product
+  float ref = 0.f, g = 0.f, miss = 0.f;
+  int target = -1;
+  if (LOGITS) {
+    target = p.target[row];
+    ref = MODE == kGrad ? p.rows.lse[row] : p.rows.ref[row];
+    if (MODE == kGrad && row < live) {
+      g = row_upstream(p.upstream, p.per_token, p.mean, p.source[row], live);
+      miss = p.rows.miss[row];
+    }
+  }
+  float sum = 0.f, far = -INFINITY;  // the sum within the window; log2 of what lies above it, against the reference
+#pragma unroll 1
+  for (int c = 0; c < 4; ++c) {
+    const int col = c_first + 32 * c;
+    float v[32];
+    tmem_ld32(acc + 32 * c, v);
+    if (c == 3) {
+      tc_fence_before();
+      mbar_arrive_remote(tempty, 0);  // the whole accumulator has been read
+    }
+    if (LOGITS) {
+      const int vcol = p.v0 + col;  // of the vocabulary
+      if (vcol + 32 > p.vocab || (target >= vcol && target < vcol + 32)) {  // past the end, or the target's own
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+          if (vcol + j >= p.vocab || vcol + j == target) v[j] = -INFINITY;
+      }
+      float e[32];
+      float s = 0.f;
+#pragma unroll
+      for (int j = 0; j < 32; ++j) {
+        e[j] = exp2_fast(fmaf(v[j], kLog2e, -ref));
+        s += e[j];
+      }
+      if (MODE == kStats || MODE == kProbs) {
+        if (s < kWindow) {
+          sum += s;
+        } else {  // against the piece's own maximum (a NaN stays one)
+          float top = v[0];
+#pragma unroll
+          for (int j = 1; j < 32; ++j) top = fmaxf(top, v[j]);
+          float t = 0.f;
+#pragma unroll
+          for (int j = 0; j < 32; ++j) t += exp2_fast((v[j] - top) * kLog2e);
+          const float here = fmaf(top, kLog2e, -ref) + log2f(t);
+          const float hi = fmaxf(far, here), lo = fminf(far, here);
+          far = here != here ? here : (far != far ? far : hi + log2f(1.0f + exp2f(lo - hi)));
+        }
+      }
+      if (MODE == kGrad) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) e[j] *= g;
+        if (target >= vcol && target < vcol + 32) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (vcol + j == target) e[j] = -miss * g;
+        }
+      }
+      if (MODE != kStats) {
+        uint32_t w[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) w[j] = pack_bf16x2(e[2 * j], e[2 * j + 1]);
+        const uint32_t tile = stg + (c & 1) * 2048u;
+        if (lane == 0) bulk_wait_read<1>();  // the tile's last store has read it
+        __syncwarp();
+        stage_bf16(tile, lane, w);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          tma_store_2d(out, tile, col, row0);
+          bulk_commit();
+        }
+      }
+    } else {
+      if (empty) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = 0.f;
+      }
+      if (MODE == kAcc) {
+        if (lane == 0) bulk_wait_read<0>();
+        __syncwarp();
+        stage_f32(stg, lane, v);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0 && col < p.hidden) {
+          const int at = part * static_cast<int>(p.rows_pad) + row0;
+          if (p.first)
+            tma_store_2d(out, stg, col, at);
+          else
+            tma_add_2d(out, stg, col, at);
+          bulk_commit();
+        }
+      } else {
+        uint32_t w[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) w[j] = pack_bf16x2(v[2 * j], v[2 * j + 1]);
+        const uint32_t tile = stg + (c & 1) * 2048u;
+        if (lane == 0) bulk_wait_read<1>();
+        __syncwarp();
+        stage_bf16(tile, lane, w);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          if (col < p.hidden && p.v0 + row0 < p.vocab) tma_store_2d(out, tile, col, p.v0 + row0);
+          bulk_commit();
+        }
+      }
+    }
+  }
+  if (MODE == kStats || MODE == kProbs) {
+    const int slot = 2 * (p.v0 / TILE + n) + half;
+    // what lies above the window is kept as minus its log2 against the reference (over 90, so never near zero)
+    float kept = sum;
+    if (far != -INFINITY) kept = far != far ? far : -(far + log2f(1.0f + sum * exp2f(-far)));
+    p.part[static_cast<int64_t>(slot) * p.rows_pad + row] = kept;
+  }
+}
+
+template <int MODE, bool REDO>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
+    vocab_product(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb,
+                  const __grid_constant__ CUtensorMap tout, const Params p) {
+  constexpr bool A_MN = MODE == kWeight;
+  constexpr bool B_MN = MODE == kWeight || MODE == kAcc;
+  if (REDO && p.state[kRedo] == 0) return;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const uint32_t sbase = smem_u32(smem);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank();
+  const int pair_id = static_cast<int>(cluster_id_x()), pairs = static_cast<int>(num_clusters_x());
+
+  const uint32_t bar0 = sbase + OFF_BAR;
+  auto bar_full = [&](int s) { return bar0 + 8u * s; };
+  auto bar_empty = [&](int s) { return bar0 + 8u * (STAGES + s); };
+  auto bar_tfull = [&](int b) { return bar0 + 8u * (2 * STAGES + b); };
+  auto bar_tempty = [&](int b) { return bar0 + 8u * (2 * STAGES + 2 + b); };
+  const uint32_t bar_drain = bar0 + 8u * (2 * STAGES + 4);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + OFF_TMEM);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(bar_full(s), 1);
+      mbar_init(bar_empty(s), 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(bar_tfull(b), 1);
+      mbar_init(bar_tempty(b), 512);  // 256 epilogue threads of each CTA
+    }
+    mbar_init(bar_drain, 1);
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(smem_u32(tmem_slot), TMEM_COLS);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  const Units w = units_of<MODE>(p, pairs);
+  const int live = p.state[kLive];
+
+  if (warp == 0) {
+    if (lane == 0) {  // ---------------------------------------------------------------------- TMA producer (each CTA)
+      tma_prefetch_desc(&ta);
+      tma_prefetch_desc(&tb);
+      int stage = 0;
+      uint32_t phase = 0;
+      uint32_t last_parity[STAGES];
+      bool issued[STAGES];
+      for (int s = 0; s < STAGES; ++s) issued[s] = false, last_parity[s] = 0;
+      bool ok = true;
+      for (int u = pair_id; u < w.total && ok; u += pairs) {
+        int m, n, part;
+        w.decode(u, m, n, part);
+        if (REDO && p.flags[m] == 0) continue;
+        const int a0 = m * TILE + 128 * static_cast<int>(rank), b0 = n * TILE + 128 * static_cast<int>(rank);
+        const int k1 = w.k_begin(part + 1);
+        for (int kb = w.k_begin(part); kb < k1; ++kb) {
+          if (!mbar_wait(bar_empty(stage), phase ^ 1)) { ok = false; break; }
+          const uint32_t fb = map_to_rank(bar_full(stage), 0);
+          const uint32_t a_dst = sbase + stage * STAGE_BYTES, b_dst = a_dst + OPERAND_BYTES;
+          const int k0 = kb * BK;
+          if (rank == 0) mbar_arrive_expect_tx(bar_full(stage), 2 * STAGE_BYTES);
+          if (A_MN) {
+            tma_load_2d_pair(a_dst, &ta, fb, a0, k0);
+            tma_load_2d_pair(a_dst + 8192, &ta, fb, a0 + 64, k0);
+          } else {
+            tma_load_2d_pair(a_dst, &ta, fb, k0, a0);
+          }
+          if (B_MN) {
+            const int kr = MODE == kAcc ? p.v0 + k0 : k0;
+            tma_load_2d_pair(b_dst, &tb, fb, b0, kr);
+            tma_load_2d_pair(b_dst + 8192, &tb, fb, b0 + 64, kr);
+          } else {
+            tma_load_2d_pair(b_dst, &tb, fb, k0, p.v0 + b0);
+          }
+          issued[stage] = true;
+          last_parity[stage] = phase;
+          if (++stage == STAGES) stage = 0, phase ^= 1;
+        }
+      }
+      if (!ok && rank == 0)
+        for (int s = 0; s < STAGES; ++s)
+          if (issued[s]) mbar_wait_drain(bar_full(s), last_parity[s]);
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && rank == 0) {  // -------------------------------------------------------- MMA issuer (the leader)
+      constexpr uint32_t IDESC = idesc_bf16(256, 256, A_MN, B_MN);
+      const uint64_t a_desc0 = A_MN ? smem_desc(sbase, 8192, 1024, 2) : smem_desc(sbase, 16, 1024, 2);
+      const uint64_t b_desc0 = B_MN ? smem_desc(sbase + OPERAND_BYTES, 8192, 1024, 2)
+                                    : smem_desc(sbase + OPERAND_BYTES, 16, 1024, 2);
+      constexpr uint32_t A_KK = A_MN ? 2048 / 16 : 32 / 16, B_KK = B_MN ? 2048 / 16 : 32 / 16;
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      int it = 0;
+      for (int u = pair_id; u < w.total && ok; u += pairs) {
+        int m, n, part;
+        w.decode(u, m, n, part);
+        if (REDO && p.flags[m] == 0) continue;
+        const int ab = it & 1;
+        if (!mbar_wait_cluster(bar_tempty(ab), ((it >> 1) & 1) ^ 1)) { ok = false; break; }
+        tc_fence_after();
+        const uint32_t d = tmem_base + ab * TILE;
+        const int k0 = w.k_begin(part), k1 = w.k_begin(part + 1);
+        for (int kb = k0; kb < k1; ++kb) {
+          if (!mbar_wait(bar_full(stage), phase)) { ok = false; break; }
+          tc_fence_after();
+          const uint64_t a_st = a_desc0 + static_cast<uint32_t>(stage) * (STAGE_BYTES / 16);
+          const uint64_t b_st = b_desc0 + static_cast<uint32_t>(stage) * (STAGE_BYTES / 16);
+          mma_bf16_pair(d, a_st, b_st, IDESC, kb != k0);
+#pragma unroll
+          for (int kk = 1; kk < BK / 16; ++kk) mma_bf16_pair(d, a_st + A_KK * kk, b_st + B_KK * kk, IDESC, 1);
+          mma_commit_pair(bar_empty(stage));
+          if (++stage == STAGES) stage = 0, phase ^= 1;
+        }
+        if (!ok) break;
+        mma_commit_pair(bar_tfull(ab));
+        ++it;
+      }
+      if (!ok) {
+        mma_commit_pair(bar_drain);
+        mbar_wait_drain(bar_drain, 0);
+      }
+    }
+  } else if (warp >= EPI_WARP0) {  // --------------------------------------------------------- epilogue (each CTA)
+    const int q = warp & 3, half = (warp - EPI_WARP0) >> 2;
+    const uint32_t stg = sbase + OFF_STG + static_cast<uint32_t>(warp - EPI_WARP0) * STG_BYTES;
+    int it = 0;
+    for (int u = pair_id; u < w.total; u += pairs) {
+      int m, n, part;
+      w.decode(u, m, n, part);
+      if (REDO && p.flags[m] == 0) continue;
+      const int ab = it & 1;
+      if (!mbar_wait(bar_tfull(ab), (it >> 1) & 1)) break;
+      tc_fence_after();
+      const uint32_t acc = tmem_base + ab * TILE + half * 128 + (static_cast<uint32_t>(32 * q) << 16);
+      epilogue<MODE>(p, &tout, m, n, part, w.k_begin(part) == w.k_begin(part + 1),
+                     m * TILE + 128 * static_cast<int>(rank) + 32 * q, half, acc, lane, stg, bar_tempty(ab), live);
+      ++it;
+    }
+    if (lane == 0) bulk_wait_all();
+  }
+
+  tc_fence_before();
+  cluster_sync();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem_base, TMEM_COLS);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------- rows
+
+// The tokens with a target, in order: source (live row -> token), slot (token -> live row, or -1), their number; the
+// losses of the ignored tokens (zero) and the state words of this call. One CTA, each thread a run of tokens: the
+// ids are 8 bytes a token and the block's scan is one, so 16,384 tokens take a few microseconds.
+__global__ void __launch_bounds__(1024) vocab_scan(const int64_t* __restrict__ targets, int64_t tokens,
+                                                  int64_t ignore, int32_t* __restrict__ source,
+                                                  int32_t* __restrict__ slot, int32_t* __restrict__ state,
+                                                  int32_t* __restrict__ flags, int row_tiles,
+                                                  float* __restrict__ token_loss) {
+  __shared__ int warp_sum[32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t per = (tokens + 1023) / 1024;
+  const int64_t t0 = min(tokens, per * threadIdx.x), t1 = min(tokens, t0 + per);
+  int mine = 0;
+  for (int64_t t = t0; t < t1; ++t) mine += targets[t] != ignore;
+  int incl = mine;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, incl, off);
+    if (lane >= off) incl += v;
+  }
+  if (lane == 31) warp_sum[warp] = incl;
+  __syncthreads();
+  if (warp == 0) {
+    int v = warp_sum[lane];
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const int o = __shfl_up_sync(0xffffffffu, v, off);
+      if (lane >= off) v += o;
+    }
+    warp_sum[lane] = v;
+  }
+  __syncthreads();
+  int at = incl - mine + (warp ? warp_sum[warp - 1] : 0);
+  for (int64_t t = t0; t < t1; ++t) {
+    const bool is = targets[t] != ignore;
+    slot[t] = is ? at : -1;
+    if (is) source[at++] = static_cast<int32_t>(t);
+    if (!is && token_loss != nullptr) token_loss[t] = 0.f;
+  }
+  for (int i = threadIdx.x; i < row_tiles; i += 1024) flags[i] = 0;
+  if (threadIdx.x < kStateInts) state[threadIdx.x] = threadIdx.x == kLive ? warp_sum[31] : 0;
+}
+
+// Each live row copied to the front of `compact`, its target and its target's logit (a float32 dot product): a warp
+// per row. The rows from the last live one to the end of its 256-row tile are zero (the head's gradient sums over
+// them). A target outside the vocabulary makes the row's reference, and with it its loss and its gradient, NaN.
+__global__ void __launch_bounds__(256) vocab_gather(const __nv_bfloat16* __restrict__ hidden, int64_t ld_hidden,
+                                                   const __nv_bfloat16* __restrict__ weight, int64_t ld_weight,
+                                                   const int64_t* __restrict__ targets, int vocab, int width,
+                                                   const int32_t* __restrict__ state,
+                                                   const int32_t* __restrict__ source, __nv_bfloat16* __restrict__ compact,
+                                                   int32_t* __restrict__ target, Rows rows) {
+  const int lane = threadIdx.x & 31;
+  const int row = blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int live = state[kLive];
+  if (row >= (live + TILE - 1) / TILE * TILE) return;
+  uint4* to = reinterpret_cast<uint4*>(compact + static_cast<int64_t>(row) * width);
+  const int vecs = width / 8;
+  if (row >= live) {
+    for (int i = lane; i < vecs; i += 32) to[i] = make_uint4(0, 0, 0, 0);
+    if (lane == 0) {
+      target[row] = -1;
+      rows.ref[row] = 0.f, rows.logit[row] = 0.f, rows.lse[row] = 0.f, rows.scale[row] = 0.f, rows.miss[row] = 0.f;
+    }
+    return;
+  }
+  const int64_t t = source[row];
+  const int64_t y = targets[t];
+  const bool inside = y >= 0 && y < vocab;
+  const uint4* h = reinterpret_cast<const uint4*>(hidden + t * ld_hidden);
+  const uint4* wr = reinterpret_cast<const uint4*>(weight + (inside ? y : 0) * ld_weight);
+  float dot = 0.f;
+  for (int i = lane; i < vecs; i += 32) {
+    const uint4 a = h[i], b = wr[i];
+    to[i] = a;
+    dot = fmaf(bf16_lo(a.x), bf16_lo(b.x), dot), dot = fmaf(bf16_hi(a.x), bf16_hi(b.x), dot);
+    dot = fmaf(bf16_lo(a.y), bf16_lo(b.y), dot), dot = fmaf(bf16_hi(a.y), bf16_hi(b.y), dot);
+    dot = fmaf(bf16_lo(a.z), bf16_lo(b.z), dot), dot = fmaf(bf16_hi(a.z), bf16_hi(b.z), dot);
+    dot = fmaf(bf16_lo(a.w), bf16_lo(b.w), dot), dot = fmaf(bf16_hi(a.w), bf16_hi(b.w), dot);
+  }
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, off);
+  if (lane == 0) {
+    if (!inside) dot = __int_as_float(0x7fc00000);
+    target[row] = inside ? static_cast<int32_t>(y) : -1;
+    rows.logit[row] = dot;
+    rows.ref[row] = dot * kLog2e;
+  }
+}
+
+// Each live row's sums over the vocabulary's tiles joined in order, its loss, and the mean or the sum over the rows
+// (by the last CTA to finish, in order). 32 rows a CTA, 32 threads a row.
+__global__ void __launch_bounds__(1024) vocab_join(const float* __restrict__ part, int slots, int64_t rows_pad,
+                                                  int32_t* __restrict__ state, int32_t* __restrict__ flags,
+                                                  const int32_t* __restrict__ source, Rows rows,
+                                                  float* __restrict__ token_loss, float* __restrict__ row_loss,
+                                                  float* __restrict__ loss, int mean) {
+  __shared__ float sums[32][33], fars[32][33];
+  __shared__ double reduce[32];
+  __shared__ bool last;
+  const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
+  const int live = state[kLive];
+  const int row = blockIdx.x * 32 + x;
+  if (row < live) {
+    float sum = 0.f, far = -INFINITY;
+    for (int s = y; s < slots; s += 32) {
+      const float v = part[static_cast<int64_t>(s) * rows_pad + row];
+      if (v < 0.f) {
+        const float hi = fmaxf(far, -v), lo = fminf(far, -v);
+        far = hi + log2f(1.0f + exp2f(lo - hi));
+      } else {
+        sum += v;  // (a NaN stays one)
+      }
+    }
+    sums[y][x] = sum, fars[y][x] = far;
+  }
+  __syncthreads();
+  if (y == 0 && row < live) {
+    float sum = 0.f, far = -INFINITY;
+    for (int i = 0; i < 32; ++i) {
+      sum += sums[i][x];
+      const float f = fars[i][x];
+      if (f != -INFINITY) {
+        const float hi = fmaxf(far, f), lo = fminf(far, f);
+        far = hi + log2f(1.0f + exp2f(lo - hi));
+      }
+    }
+    // the reference was rounded to a multiple of log 2: what the rounding took is put back
+    const float ref = rows.ref[row], logit = rows.logit[row];
+    const float off = fmaf(logit, kLog2e, -ref);
+    float value;
+    if (far == -INFINITY) {
+      sum *= exp2f(-off);
+      const float z = 1.0f + sum;
+      value = log1pf(sum);
+      rows.lse[row] = fmaf(logit, kLog2e, log2f(z));
+      rows.scale[row] = exp2f(-off) / z;
+      rows.miss[row] = sum / z;
+    } else {
+      const float more = far + log2f(1.0f + (1.0f + sum) * exp2f(-far)) - off;
+      value = more * kLn2;
+      const float lse = fmaf(logit, kLog2e, more);
+      rows.lse[row] = lse;
+      rows.ref[row] = lse;
+      rows.scale[row] = 1.0f;
+      rows.miss[row] = 1.0f - exp2f(-more);
+      flags[row / TILE] = 1;
+      state[kRedo] = 1;
+    }
+    if (token_loss != nullptr) token_loss[source[row]] = value;
+    else row_loss[row] = value;
+  }
+  if (token_loss != nullptr) return;
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) last = atomicAdd(&state[kDone], 1) == static_cast<int>(gridDim.x) - 1;
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  double total = 0.0;
+  for (int i = threadIdx.x; i < live; i += 1024) total += static_cast<double>(__ldcg(row_loss + i));
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) total += __shfl_xor_sync(0xffffffffu, total, off);
+  if (x == 0) reduce[y] = total;
+  __syncthreads();
+  if (y == 0) {
+    total = reduce[x];
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) total += __shfl_xor_sync(0xffffffffu, total, off);
+    if (x == 0) *loss = static_cast<float>(mean ? total / max(live, 1) : total);
+  }
+}
+
+// dh of every token from its row's planes: g (scale sum_planes - miss W_y), or the planes' sum alone where the
+// product was over the gradient itself (weight == nullptr); zero for ignored tokens. A warp per token.
+__global__ void __launch_bounds__(256) vocab_finish(const float* __restrict__ acc, int pairs, int planes,
+                                                   int64_t rows_pad, int width, int64_t tokens,
+                                                   const int32_t* __restrict__ state, const int32_t* __restrict__ slot,
+                                                   const int32_t* __restrict__ target, Rows rows,
+                                                   const __nv_bfloat16* __restrict__ weight, int64_t ld_weight,
+                                                   const float* __restrict__ upstream, int per_token, int mean,
+                                                   __nv_bfloat16* __restrict__ d_hidden) {
+  const int lane = threadIdx.x & 31;
+  const int64_t t = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  if (t >= tokens) return;
+  uint4* to = reinterpret_cast<uint4*>(d_hidden + t * width);
+  const int vecs = width / 8;
+  const int row = slot[t];
+  if (row < 0) {
+    for (int i = lane; i < vecs; i += 32) to[i] = make_uint4(0, 0, 0, 0);
+    return;
+  }
+  const int live = state[kLive];
+  const int parts = depth_parts((live + TILE - 1) / TILE * ((width + TILE - 1) / TILE), pairs, planes);
+  float a = 1.f, b = 0.f;
+  const uint4* wr = nullptr;
+  if (weight != nullptr) {
+    const float g = row_upstream(upstream, per_token, mean, static_cast<int>(t), live);
+    a = g * rows.scale[row], b = g * rows.miss[row];
+    const int y = target[row];
+    wr = reinterpret_cast<const uint4*>(weight + static_cast<int64_t>(y < 0 ? 0 : y) * ld_weight);
+  }
+  for (int i = lane; i < vecs; i += 32) {
+    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < parts; ++s) {
+      const float4* from = reinterpret_cast<const float4*>(acc + (s * rows_pad + row) * width) + 2 * i;
+      const float4 u = __ldcs(from), w = __ldcs(from + 1);
+      v[0] += u.x, v[1] += u.y, v[2] += u.z, v[3] += u.w, v[4] += w.x, v[5] += w.y, v[6] += w.z, v[7] += w.w;
+    }
+    if (wr != nullptr) {
+      const uint4 k = wr[i];
+      v[0] = a * v[0] - b * bf16_lo(k.x), v[1] = a * v[1] - b * bf16_hi(k.x);
+      v[2] = a * v[2] - b * bf16_lo(k.y), v[3] = a * v[3] - b * bf16_hi(k.y);
+      v[4] = a * v[4] - b * bf16_lo(k.z), v[5] = a * v[5] - b * bf16_hi(k.z);
+      v[6] = a * v[6] - b * bf16_lo(k.w), v[7] = a * v[7] - b * bf16_hi(k.w);
+    }
+    to[i] = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
+                       pack_bf16x2(v[6], v[7]));
+  }
+}
+
+template <int MODE, bool REDO>
+static int launch(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& out, const Params& p, int pairs,
+                  cudaStream_t s) {
+  auto kern = vocab_product<MODE, REDO>;
+  static uint64_t configured = 0;  // per device: a function's attributes are set on the current one
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess) return cudaGetLastError(), MEEP2B_ERR_LAUNCH;
+  if (device >= 64 || !((configured >> device) & 1)) {
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES) != cudaSuccess) {
+      cudaGetLastError();
+      return MEEP2B_ERR_LAUNCH;
+    }
+    if (device < 64) configured |= uint64_t(1) << device;
+  }
+  kern<<<2 * pairs, THREADS, SMEM_BYTES, s>>>(a, b, out, p);
+  return launch_status();
+}
+
+static int map_bf16(CUtensorMap* map, const void* base, int64_t inner, int64_t rows, int64_t ld, uint32_t box_inner,
+                    uint32_t box_rows, CUtensorMapSwizzle swizzle) {
+  const uint64_t dims[2] = {static_cast<uint64_t>(inner), static_cast<uint64_t>(rows)};
+  const uint64_t strides[1] = {static_cast<uint64_t>(ld) * 2};
+  const uint32_t box[2] = {box_inner, box_rows};
+  return encode_tiled(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, base, dims, strides, box, swizzle);
+}
+
+}  // namespace vocab
+}  // namespace meep2b
+
+using namespace meep2b;
+
+namespace {
+
+constexpr int64_t kPieceBytes = int64_t(1) << 30;  // a piece's buffer; see meep2b_linear_ce_plan
+constexpr int64_t kPlaneBytes = int64_t(1) << 29;
+constexpr int kMostPlanes = 16;
+
+int pairs_of_device(int* pairs) {
+  int device = 0, sms = 0;
+  if (cudaGetDevice(&device) != cudaSuccess ||
+      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) {
+    cudaGetLastError();
+    return MEEP2B_ERR_LAUNCH;
+  }
+  *pairs = sms / 2 > 0 ? sms / 2 : 1;
+  return MEEP2B_OK;
+}
+
+int check_linear_ce(const meep2b_linear_ce* a, bool forward) {
+  if (a == nullptr || a->tokens < 0 || a->hidden_size < 1 || a->vocab < 1) return MEEP2B_ERR_SHAPE;
+  if (a->tokens > (1 << 24) || a->vocab > (1 << 24) || a->hidden_size > (1 << 20)) return MEEP2B_ERR_SHAPE;
+  if (a->hidden_size % 8 || a->ld_weight % 8 || a->ld_weight < a->hidden_size || !aligned16(a->weight))
+    return MEEP2B_ERR_ALIGN;
+  if (forward && (a->ld_hidden % 8 || !aligned16(a->hidden))) return MEEP2B_ERR_ALIGN;
+  if (a->reduction < 0 || a->reduction > 2) return MEEP2B_ERR_UNSUPPORTED;
+  if (a->rows_pad != (a->tokens + 255) / 256 * 256 || a->piece_cols % vocab::TILE || a->planes < 0)
+    return MEEP2B_ERR_SHAPE;
+  return MEEP2B_OK;
+}
+
+vocab::Rows rows_of(const meep2b_linear_ce* a) {
+  float* f = a->row_values;
+  const int64_t n = a->rows_pad;
+  return vocab::Rows{f, f + n, f + 2 * n, f + 3 * n, f + 4 * n};
+}
+
+vocab::Params params_of(const meep2b_linear_ce* a) {
+  vocab::Params p = {};
+  p.state = a->state, p.flags = a->flags, p.target = a->target, p.source = a->source, p.rows = rows_of(a);
+  p.part = a->part, p.rows_pad = a->rows_pad, p.upstream = a->upstream;
+  p.per_token = a->reduction == MEEP2B_REDUCE_NONE, p.mean = a->reduction == MEEP2B_REDUCE_MEAN;
+  p.vocab = static_cast<int>(a->vocab), p.hidden = static_cast<int>(a->hidden_size), p.planes = a->planes;
+  return p;
+}
+
+struct CeMaps {
+  CUtensorMap rows, rows_mn, head, head_mn, piece, piece_mn, piece_out, acc, d_weight;
+};
+
+int maps_of(const meep2b_linear_ce* a, CeMaps* m, bool acc, bool d_weight) {
+  using vocab::map_bf16;
+  const int64_t H = a->hidden_size;
+  MEEP2B_TRY(map_bf16(&m->rows, a->compact, H, a->rows_pad, H, 64, 128, CU_TENSOR_MAP_SWIZZLE_128B));
+  MEEP2B_TRY(map_bf16(&m->head, a->weight, H, a->vocab, a->ld_weight, 64, 128, CU_TENSOR_MAP_SWIZZLE_128B));
+  if (a->piece != nullptr) {
+    MEEP2B_TRY(map_bf16(&m->piece, a->piece, a->piece_cols, a->rows_pad, a->piece_cols, 64, 128,
+                        CU_TENSOR_MAP_SWIZZLE_128B));
+    MEEP2B_TRY(map_bf16(&m->piece_out, a->piece, a->piece_cols, a->rows_pad, a->piece_cols, 32, 32,
+                        CU_TENSOR_MAP_SWIZZLE_64B));
+  } else {
+    m->piece_out = m->rows;  // not used
+  }
+  if (acc) {
+    MEEP2B_TRY(map_bf16(&m->head_mn, a->weight, H, a->vocab, a->ld_weight, 64, 64, CU_TENSOR_MAP_SWIZZLE_128B));
+    const uint64_t dims[2] = {static_cast<uint64_t>(H), static_cast<uint64_t>(a->planes * a->rows_pad)};
+    const uint64_t strides[1] = {static_cast<uint64_t>(H) * 4};
+    const uint32_t box[2] = {32, 32};
+    MEEP2B_TRY(encode_tiled(&m->acc, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, a->acc, dims, strides, box,
+                            CU_TENSOR_MAP_SWIZZLE_128B));
+  }
+  if (d_weight) {
+    MEEP2B_TRY(map_bf16(&m->rows_mn, a->compact, H, a->rows_pad, H, 64, 64, CU_TENSOR_MAP_SWIZZLE_128B));
+    MEEP2B_TRY(map_bf16(&m->piece_mn, a->piece, a->piece_cols, a->rows_pad, a->piece_cols, 64, 64,
+                        CU_TENSOR_MAP_SWIZZLE_128B));
+    MEEP2B_TRY(map_bf16(&m->d_weight, a->d_weight, H, a->vocab, H, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B));
+  }
+  return MEEP2B_OK;
+}
+
+// The vocabulary's pieces: first column, column tiles and depth of each.
+template <typename F>
+int each_piece(const meep2b_linear_ce* a, vocab::Params p, F f) {
+  const int64_t cols = a->piece_cols > 0 ? a->piece_cols : (a->vocab + 255) / 256 * 256;
+  for (int64_t v0 = 0; v0 < a->vocab; v0 += cols) {
+    const int64_t width = a->vocab - v0 < cols ? a->vocab - v0 : cols;
+    p.v0 = static_cast<int>(v0);
+    p.piece_tiles = static_cast<int>((width + vocab::TILE - 1) / vocab::TILE);
+    p.k_total = static_cast<int>(width);
+    p.first = v0 == 0;
+    MEEP2B_TRY(f(p));
+  }
+  return MEEP2B_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int meep2b_linear_ce_plan(int64_t tokens, int64_t hidden_size, int64_t vocab, int64_t* rows_pad, int64_t* piece_cols,
+                          int32_t* planes) {
+  if (tokens < 0 || hidden_size < 1 || vocab < 1 || tokens > (1 << 24) || vocab > (1 << 24) || hidden_size > (1 << 20))
+    return MEEP2B_ERR_SHAPE;
+  *rows_pad = (tokens + 255) / 256 * 256;
+  const int64_t rows = *rows_pad > 0 ? *rows_pad : 256;
+  const int64_t tiles = (vocab + 255) / 256;
+  int64_t most = kPieceBytes / (rows * 2 * 256);
+  most = most < 1 ? 1 : most;
+  const int64_t pieces = (tiles + most - 1) / most;
+  *piece_cols = (tiles + pieces - 1) / pieces * 256;
+  int64_t p = kPlaneBytes / (rows * hidden_size * 4);
+  p = p < 1 ? 1 : (p > kMostPlanes ? kMostPlanes : p);
+  *planes = static_cast<int32_t>(p);
+  return MEEP2B_OK;
+}
+
+int meep2b_linear_ce_forward(const meep2b_linear_ce* a, void* stream) {
+  MEEP2B_TRY(check_linear_ce(a, true));
+  if (a->loss == nullptr || a->state == nullptr || a->part == nullptr) return MEEP2B_ERR_SHAPE;
+  cudaStream_t s = as_stream(stream);
+  MEEP2B_TRY(bind_stream_device(s));
+  const bool per_token = a->reduction == MEEP2B_REDUCE_NONE;
+  const bool grad = a->acc != nullptr;
+  if (grad && (a->piece == nullptr || a->planes < 1)) return MEEP2B_ERR_SHAPE;
+  const vocab::Rows rows = rows_of(a);
+  const int row_tiles = static_cast<int>(a->rows_pad / vocab::TILE);
+  vocab::vocab_scan<<<1, 1024, 0, s>>>(a->targets, a->tokens, a->ignore_index, a->source, a->slot, a->state, a->flags,
+                                       row_tiles, per_token ? a->loss : nullptr);
+  MEEP2B_TRY(launch_status());
+  const int slots = 2 * static_cast<int>((a->vocab + vocab::TILE - 1) / vocab::TILE);
+  if (a->tokens > 0) {
+    vocab::vocab_gather<<<static_cast<unsigned>(a->rows_pad / 8), 256, 0, s>>>(
+        static_cast<const __nv_bfloat16*>(a->hidden), a->ld_hidden, static_cast<const __nv_bfloat16*>(a->weight),
+        a->ld_weight, a->targets, static_cast<int>(a->vocab), static_cast<int>(a->hidden_size), a->state, a->source,
+        static_cast<__nv_bfloat16*>(a->compact), a->target, rows);
+    MEEP2B_TRY(launch_status());
+    int pairs = 0;
+    MEEP2B_TRY(pairs_of_device(&pairs));
+    CeMaps m;
+    MEEP2B_TRY(maps_of(a, &m, grad, false));
+    MEEP2B_TRY(each_piece(a, params_of(a), [&](const vocab::Params& p) -> int {
+      if (!grad) return vocab::launch<vocab::kStats, false>(m.rows, m.head, m.piece_out, p, pairs, s);
+      MEEP2B_TRY((vocab::launch<vocab::kProbs, false>(m.rows, m.head, m.piece_out, p, pairs, s)));
+      return vocab::launch<vocab::kAcc, false>(m.piece, m.head_mn, m.acc, p, pairs, s);
+    }));
+  }
+  const unsigned join = static_cast<unsigned>(a->tokens > 0 ? (a->tokens + 31) / 32 : 1);
+  vocab::vocab_join<<<join, 1024, 0, s>>>(a->part, slots, a->rows_pad, a->state, a->flags, a->source, rows,
+                                          per_token ? a->loss : nullptr, a->row_loss, a->loss,
+                                          a->reduction == MEEP2B_REDUCE_MEAN);
+  MEEP2B_TRY(launch_status());
+  if (grad && a->tokens > 0) {
+    int pairs = 0;
+    MEEP2B_TRY(pairs_of_device(&pairs));
+    CeMaps m;
+    MEEP2B_TRY(maps_of(a, &m, true, false));
+    MEEP2B_TRY(each_piece(a, params_of(a), [&](const vocab::Params& p) -> int {
+      MEEP2B_TRY((vocab::launch<vocab::kReprobs, true>(m.rows, m.head, m.piece_out, p, pairs, s)));
+      return vocab::launch<vocab::kAcc, true>(m.piece, m.head_mn, m.acc, p, pairs, s);
+    }));
+  }
+  return MEEP2B_OK;
+}
+
+int meep2b_linear_ce_backward(const meep2b_linear_ce* a, void* stream) {
+  MEEP2B_TRY(check_linear_ce(a, false));
+  if (a->upstream == nullptr || (a->d_hidden == nullptr && a->d_weight == nullptr)) return MEEP2B_ERR_SHAPE;
+  if (a->d_hidden != nullptr && (a->acc == nullptr || a->planes < 1)) return MEEP2B_ERR_SHAPE;
+  if ((a->d_hidden && !aligned16(a->d_hidden)) || (a->d_weight && !aligned16(a->d_weight))) return MEEP2B_ERR_ALIGN;
+  cudaStream_t s = as_stream(stream);
+  MEEP2B_TRY(bind_stream_device(s));
+  int pairs = 0;
+  MEEP2B_TRY(pairs_of_device(&pairs));
+  const bool recompute = a->d_weight != nullptr;  // else the forward pass left dh's planes
+  if (recompute && a->piece == nullptr) return MEEP2B_ERR_SHAPE;
+  if (recompute && a->tokens == 0) {
+    const cudaError_t e = cudaMemsetAsync(a->d_weight, 0, static_cast<size_t>(a->vocab) * a->hidden_size * 2, s);
+    return e == cudaSuccess ? MEEP2B_OK : (cudaGetLastError(), MEEP2B_ERR_LAUNCH);
+  }
+  if (recompute) {
+    CeMaps m;
+    MEEP2B_TRY(maps_of(a, &m, a->d_hidden != nullptr, true));
+    MEEP2B_TRY(each_piece(a, params_of(a), [&](const vocab::Params& p) -> int {
+      MEEP2B_TRY((vocab::launch<vocab::kGrad, false>(m.rows, m.head, m.piece_out, p, pairs, s)));
+      if (a->d_hidden != nullptr)
+        MEEP2B_TRY((vocab::launch<vocab::kAcc, false>(m.piece, m.head_mn, m.acc, p, pairs, s)));
+      return vocab::launch<vocab::kWeight, false>(m.piece_mn, m.rows_mn, m.d_weight, p, pairs, s);
+    }));
+  }
+  if (a->d_hidden != nullptr && a->tokens > 0) {
+    const vocab::Params p = params_of(a);
+    vocab::vocab_finish<<<static_cast<unsigned>((a->tokens + 7) / 8), 256, 0, s>>>(
+        a->acc, pairs, a->planes, a->rows_pad, static_cast<int>(a->hidden_size), a->tokens, a->state, a->slot,
+        a->target, p.rows, recompute ? nullptr : static_cast<const __nv_bfloat16*>(a->weight), a->ld_weight,
+        a->upstream, p.per_token, p.mean, static_cast<__nv_bfloat16*>(a->d_hidden));
+    MEEP2B_TRY(launch_status());
+  }
+  return MEEP2B_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,39 @@
+"""The fine-tuning step's operators without a GPU: the buffers the vocabulary loss plans, and the refusal to run on the
+CPU."""
+
+import pytest
+import torch
+
+import meepsquared_b200 as mb
+from meepsquared_b200 import _loss
+
+
+@pytest.mark.parametrize("tokens", [1, 255, 256, 257, 4096, 16384, 1 << 20])
+@pytest.mark.parametrize("vocab", [1, 256, 257, 32003, 131072, 262144])
+@pytest.mark.parametrize("hidden", [8, 2048, 8192])
+def test_the_plan_of_the_vocabulary_loss(tokens, vocab, hidden):
+    rows, cols, planes = _loss._plan(tokens, hidden, vocab)
+    assert rows % 256 == 0 and tokens <= rows < tokens + 256
+    assert cols % 256 == 0 and 256 <= cols < vocab + 256
+    assert cols == 256 or rows * cols * 2 <= 1 << 30
+    assert 1 <= planes <= 16 and (planes == 1 or planes * rows * hidden * 4 <= 1 << 29)
+    pieces = -(-vocab // cols)
+    assert pieces * cols - vocab < pieces * 256 + 256  # the pieces are about equal
+
+
+def test_sizes_beyond_the_entry_point_are_refused():
+    with pytest.raises(ValueError):
+        _loss._plan(1 << 25, 64, 1000)
+    with pytest.raises(ValueError):
+        _loss._plan(16, 0, 1000)
+
+
+def test_no_cpu_fallback():
+    x = torch.zeros((4, 64), dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        mb.linear_cross_entropy(x, x, torch.zeros(4, dtype=torch.int64))
+    with pytest.raises(RuntimeError, match="CUDA"):
+        mb.balance_loss(x, 2)
+    q = torch.zeros((1, 4, 2, 64))
+    with pytest.raises(RuntimeError, match="CUDA"):
+        mb.qk_norm_rope(q, q, torch.ones(64), torch.ones(64), torch.ones(4, 32), torch.ones(4, 32))

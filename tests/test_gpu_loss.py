@@ -1,0 +1,305 @@
+"""linear_cross_entropy against softmax cross entropy in float64: losses, the hidden states' gradient and the head's.
+
+Tolerances, with d = (H / 16 + 16) 2^-23 max_tv sum_i |h_ti W_vi|, what a float32 sum of H products (in tensor-core
+steps of 16, each rounded or cut) can be off, for a logit:
+  loss   2 d for the logits that enter it, and 2^-20 of itself for its logarithm and its sum over the vocabulary;
+  dh     the probabilities are rounded to bf16 (2^-8 of each, of which the sum over the vocabulary keeps at most
+         2^-8 sum_v p_v |W_v|) and carry their logits' error (2 d); one bf16 rounding at the end;
+  dW     the same with the sum over the tokens.
+What float32 cannot hold is zero: probabilities below 2^-126, so that dh and dW may miss FLOOR."""
+
+import pytest
+import torch
+
+import meepsquared_b200 as mb
+from meepsquared_b200 import _lib, _loss
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+HALF_ULP = 1.1 * 2.0 ** -8  # of a bf16 rounding, and a tenth for the float32 arithmetic around it
+
+FLOOR = 1e-35  # 2^-126 times a vocabulary's weights
+
+
+def inputs(tokens, hidden, vocab, seed=0, scale=1.0, ignored=0.0):
+    gen = torch.Generator().manual_seed(seed)
+    h = (scale * torch.randn((tokens, hidden), generator=gen)).to(DEV, torch.bfloat16)
+    w = (torch.randn((vocab, hidden), generator=gen) * hidden ** -0.5).to(DEV, torch.bfloat16)
+    t = torch.randint(0, vocab, (tokens,), generator=gen).to(DEV)
+    if ignored:
+        t[(torch.rand((tokens,), generator=gen) < ignored).to(DEV)] = -100
+    return h, w, t
+
+
+def formula(h, w, t, upstream):
+    """Losses, dh, dW in float64 for per-token upstream gradients, and the tolerances of each."""
+    h, w, live = h.double(), w.double(), t != -100
+    z = h[live] @ w.t()
+    y = t[live]
+    at = torch.arange(y.numel(), device=h.device)
+    lse = torch.logsumexp(z, 1)
+    losses = torch.zeros(t.numel(), dtype=torch.float64, device=h.device)
+    losses[live] = lse - z[at, y]
+    p = torch.exp(z - lse[:, None])
+    g = upstream.double()[live, None]
+    dz = p.clone()
+    dz[at, y] -= 1.0
+    dz *= g
+    dh = torch.zeros_like(h)
+    dh[live] = dz @ w
+    dw = dz.t() @ h[live]
+    d = (h.shape[1] / 16 + 16) * 2.0 ** -23 * float((h[live].abs() @ w.abs().t()).max()) if y.numel() else 0.0
+    each = HALF_ULP + 2 * d
+    tol_h = torch.zeros_like(h)
+    mass = p * g.abs()
+    mass[at, y] = dz[at, y].abs()
+    tol_h[live] = each * (mass @ w.abs())
+    tol_h += HALF_ULP * dh.abs() + FLOOR
+    tol_w = each * (mass.t() @ h[live].abs()) + HALF_ULP * dw.abs() + FLOOR
+    return losses, dh, dw, 2 * d + 2.0 ** -20 * losses.abs(), tol_h, tol_w
+
+
+def within(got, want, tol, name):
+    got = got.double()
+    assert got.shape == want.shape, name
+    over = (got - want).abs() - tol
+    assert torch.isfinite(got).all() and float(over.detach().max()) <= 0, \
+        f"{name}: {float(over.detach().max()):.3g} over, {int((over > 0).sum())} of {over.numel()}"
+
+
+def check(h, w, t, reduction, head, seed=3):
+    n = t.numel()
+    up = torch.randn((n,), generator=torch.Generator().manual_seed(seed)).to(DEV) if reduction == "none" else None
+    live = int((t != -100).sum())
+    per = up if up is not None else torch.full((n,), 1.0 / max(1, live) if reduction == "mean" else 1.0, device=DEV)
+    losses, dh, dw, tol, tol_h, tol_w = formula(h, w, t, per)
+    h, w = h.detach().requires_grad_(), w.detach().requires_grad_(head)
+    loss = mb.linear_cross_entropy(h, w, t, reduction=reduction)
+    if reduction == "none":
+        within(loss, losses, tol, "losses")
+        loss.backward(up)
+    else:
+        share = max(1, live) if reduction == "mean" else 1
+        assert abs(float(loss.detach()) - float(losses.sum()) / share) <= float(tol.sum()) / share + 1e-7 * abs(float(loss.detach()))
+        loss.backward()
+    within(h.grad, dh, tol_h, "dh")
+    if head:
+        within(w.grad, dw, tol_w, "dw")
+    else:
+        assert w.grad is None
+    with torch.no_grad():
+        again = mb.linear_cross_entropy(h, w, t, reduction=reduction)
+    assert torch.equal(again, loss.detach())
+    assert _lib.device_error(0) == 0
+
+
+@pytest.mark.parametrize("head", [False, True], ids=["frozen", "trained"])
+@pytest.mark.parametrize("tokens,hidden,vocab", [(1, 8, 1), (1, 64, 7), (2, 72, 256), (37, 200, 257), (255, 64, 1000),
+                                                 (257, 128, 513), (300, 512, 5003), (700, 264, 2048)])
+def test_losses_and_gradients(tokens, hidden, vocab, head):
+    h, w, t = inputs(tokens, hidden, vocab)
+    check(h, w, t, "none", head)
+
+
+@pytest.mark.parametrize("head", [False, True], ids=["frozen", "trained"])
+@pytest.mark.parametrize("reduction", ["none", "mean", "sum"])
+@pytest.mark.parametrize("ignored", [0.3, 0.97, 1.1], ids=["some", "most", "all"])
+def test_ignored_tokens(reduction, ignored, head):
+    h, w, t = inputs(500, 136, 777, ignored=ignored)
+    check(h, w, t, reduction, head)
+
+
+@pytest.mark.parametrize("head", [False, True], ids=["frozen", "trained"])
+def test_what_ignored_tokens_hold_does_not_matter(head):
+    h, w, t = inputs(300, 64, 600, ignored=0.5)
+    clean = [x.clone() for x in (h, w, t)]
+    h[t == -100] = float("nan")
+    h[int((t == -100).nonzero()[0])] = float("inf")
+    outs = []
+    for a, b in ((clean[0], clean[1]), (h, w)):
+        a, b = a.detach().requires_grad_(), b.detach().requires_grad_(head)
+        loss = mb.linear_cross_entropy(a, b, t)
+        loss.backward()
+        outs.append((loss.detach(), a.grad, b.grad))
+    for x, y in zip(*outs):
+        assert x is None or torch.equal(x, y)
+
+
+@pytest.mark.parametrize("head", [False, True], ids=["frozen", "trained"])
+@pytest.mark.parametrize("planes", [1, 3, 16])
+@pytest.mark.parametrize("piece_cols", [256, 768])
+def test_pieces_and_planes(monkeypatch, piece_cols, planes, head):
+    plan = _loss._plan
+
+    def small(tokens, size, vocab):
+        return plan(tokens, size, vocab)[0], piece_cols, planes
+
+    monkeypatch.setattr(_loss, "_plan", small)
+    h, w, t = inputs(600, 192, 2000, ignored=0.2)
+    check(h, w, t, "none", head)
+
+
+@pytest.mark.parametrize("pieces", [False, True], ids=["whole", "pieces"])
+def test_targets_far_below_the_largest_logit(monkeypatch, pieces):
+    """Logits hundreds above the target's: beyond the window of the target's own reference, in some rows of some
+    tiles (the others keep theirs), and far below it."""
+    if pieces:
+        plan = _loss._plan
+        monkeypatch.setattr(_loss, "_plan", lambda *a: (plan(*a)[0], 512, 2))
+    h, w, t = inputs(700, 64, 1500)
+    far = torch.arange(700, device=DEV) % 97 == 5
+    h[far] *= 200.0   # logits of +-600 or so
+    h[600:] *= 30.0   # around the window's edge
+    check(h, w, t, "none", False)
+    check(h, w, t, "none", True)
+
+
+def test_a_target_far_above_the_others():
+    h, w, t = inputs(64, 64, 300)
+    h = (w[t].float() * 300.0).to(torch.bfloat16)
+    check(h, w, t, "none", False)
+
+
+@pytest.mark.parametrize("head", [False, True], ids=["frozen", "trained"])
+def test_a_target_outside_the_vocabulary_is_nan_alone(head):
+    h, w, t = inputs(40, 64, 100)
+    t[3], t[17] = 100, -5
+    h, w = h.requires_grad_(), w.requires_grad_(head)
+    loss = mb.linear_cross_entropy(h, w, t, reduction="none")
+    bad = torch.zeros(40, dtype=torch.bool, device=DEV)
+    bad[[3, 17]] = True
+    assert torch.equal(torch.isnan(loss), bad)
+    loss.sum().backward()
+    assert torch.equal(torch.isnan(h.grad).all(1), bad) and torch.equal(torch.isnan(h.grad).any(1), bad)
+
+
+def test_infinite_hidden_states_make_their_own_token_nan():
+    h, w, t = inputs(300, 64, 900)
+    h[7, 3] = float("inf")
+    h.requires_grad_()
+    loss = mb.linear_cross_entropy(h, w, t, reduction="none")
+    assert torch.isnan(loss).nonzero().flatten().tolist() == [7]
+    loss.sum().backward()
+    assert torch.isnan(h.grad).any(1).nonzero().flatten().tolist() == [7]
+
+
+def test_strides_offsets_and_shapes():
+    h, w, t = inputs(6 * 35, 64, 500, ignored=0.1)
+    want = mb.linear_cross_entropy(h, w, t, reduction="none")
+    wide = torch.zeros((210, 96), dtype=torch.bfloat16, device=DEV)
+    wide[:, 16:80] = h
+    head = torch.zeros((500, 72), dtype=torch.bfloat16, device=DEV)
+    head[:, 8:] = w
+    odd = torch.zeros((210 * 64 + 1,), dtype=torch.bfloat16, device=DEV)
+    odd[1:] = h.reshape(-1)
+    for a, b in ((wide[:, 16:80], head[:, 8:]), (odd[1:].view(210, 64), w), (h.t().contiguous().t(), w.t().contiguous().t())):
+        assert torch.equal(mb.linear_cross_entropy(a, b, t, reduction="none"), want)
+    shaped = mb.linear_cross_entropy(h.view(6, 35, 64), w, t.view(6, 35).int(), reduction="none")
+    assert torch.equal(shaped, want.view(6, 35))
+    x = wide[:, 16:80].detach().view(6, 35, 64).requires_grad_()
+    mb.linear_cross_entropy(x, w, t.view(6, 35), reduction="sum").backward()
+    y = h.detach().requires_grad_()
+    mb.linear_cross_entropy(y, w, t, reduction="sum").backward()
+    assert torch.equal(x.grad.reshape(210, 64), y.grad)
+
+
+@pytest.mark.parametrize("reduction", ["none", "mean", "sum"])
+def test_no_tokens(reduction):
+    h = torch.zeros((0, 64), dtype=torch.bfloat16, device=DEV, requires_grad=True)
+    w = torch.ones((10, 64), dtype=torch.bfloat16, device=DEV, requires_grad=True)
+    loss = mb.linear_cross_entropy(h, w, torch.zeros((0,), dtype=torch.int64, device=DEV), reduction=reduction)
+    assert loss.dtype == torch.float32 and tuple(loss.shape) == ((0,) if reduction == "none" else ())
+    loss.sum().backward()
+    assert h.grad.shape == h.shape and not w.grad.any()
+
+
+@pytest.mark.parametrize("head", [False, True], ids=["frozen", "trained"])
+def test_the_gradient_is_the_differences_slope(head):
+    """(f(h + e d) - f(h - e d)) / 2e along a direction, every point exact in bf16. The third-order term of a log-sum
+    along steps of e |logit change| ~ 0.05 is below 0.1%, the gradient's bf16 roundings 2^-8 of its terms."""
+    gen = torch.Generator().manual_seed(5)
+    h = (torch.randint(-64, 64, (32, 64), generator=gen) / 64.0).to(DEV, torch.bfloat16)
+    w = (torch.randint(-32, 32, (200, 64), generator=gen) / 64.0).to(DEV, torch.bfloat16)
+    t = torch.randint(0, 200, (32,), generator=gen).to(DEV)
+    h.requires_grad_(), w.requires_grad_(head)
+    mb.linear_cross_entropy(h, w, t, reduction="sum").backward()
+    x = w if head else h
+    sign = torch.sign(x.grad.float())
+    e = 2.0 ** -7
+    step = (sign * e).to(torch.bfloat16)
+    with torch.no_grad():
+        up, down = x + step, x - step
+        assert torch.equal(up.float(), x.float() + sign * e) and torch.equal(down.float(), x.float() - sign * e)
+        f = [mb.linear_cross_entropy(*((h, v) if head else (v, w)), t, reduction="none").double().sum() for v in (up, down)]
+    slope = float(f[0] - f[1]) / (2 * e)
+    along = float((x.grad.double() * sign).sum())
+    assert abs(slope - along) <= 0.01 * abs(along)
+
+
+def test_again_and_on_another_stream():
+    h, w, t = inputs(900, 128, 3001, ignored=0.2)
+    first = None
+    side = torch.cuda.Stream()
+    for stream in (torch.cuda.current_stream(), torch.cuda.current_stream(), side):
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            a, b = h.detach().requires_grad_(), w.detach().requires_grad_()
+            loss = mb.linear_cross_entropy(a, b, t)
+            loss.backward(retain_graph=True)
+            kept = a.grad.clone(), b.grad.clone()
+            a.grad = b.grad = None
+            loss.backward()
+            got = loss.detach(), a.grad, b.grad
+        torch.cuda.synchronize()
+        assert torch.equal(kept[0], got[1]) and torch.equal(kept[1], got[2])
+        if first is None:
+            first = got
+        assert all(torch.equal(x, y) for x, y in zip(first, got))
+
+
+def test_one_gradient_without_the_other():
+    h, w, t = inputs(300, 64, 700)
+    both = [h.detach().requires_grad_(), w.detach().requires_grad_()]
+    mb.linear_cross_entropy(*both, t).backward()
+    alone = w.detach().requires_grad_()
+    mb.linear_cross_entropy(h, alone, t).backward()
+    assert torch.equal(alone.grad, both[1].grad)
+
+
+def test_captured_in_a_graph():
+    h, w, t = inputs(300, 64, 700, ignored=0.2)
+    h.requires_grad_()
+
+    def step():
+        loss = mb.linear_cross_entropy(h, w, t)
+        return loss.detach(), torch.autograd.grad(loss, h)[0]
+
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        want = step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    graph.replay()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_refusals():
+    h, w, t = inputs(8, 64, 20)
+    with pytest.raises(ValueError, match="targets"):
+        mb.linear_cross_entropy(h, w, t[:7])
+    with pytest.raises(ValueError, match="head"):
+        mb.linear_cross_entropy(h, w[:, :56], t)
+    with pytest.raises(ValueError, match="reduction"):
+        mb.linear_cross_entropy(h, w, t, reduction="max")
+    with pytest.raises(ValueError, match="multiple of 8"):
+        mb.linear_cross_entropy(h[:, :60], w[:, :60], t)
+    with pytest.raises(TypeError, match="bf16"):
+        mb.linear_cross_entropy(h.float(), w, t)
+    with pytest.raises(TypeError, match="targets"):
+        mb.linear_cross_entropy(h, w, t.float())
+    with pytest.raises(ValueError, match="devices"):
+        mb.linear_cross_entropy(h, w.cpu(), t)
