@@ -391,7 +391,7 @@ typedef struct meep2b_linear_ce {
   int32_t reduction;       /* enum meep2b_reduction */
   int32_t planes;          /* of acc */
   int64_t rows_pad;        /* tokens up to a multiple of 256 */
-  int64_t piece_cols;      /* columns of a vocabulary piece, a multiple of 256; 0 with piece == NULL: one piece */
+  int64_t piece_cols;      /* columns of a vocabulary piece, a multiple of 256; forward, for the loss alone: 0 */
   /* written by the forward pass, read by the backward pass */
   int32_t* state;          /* 8 */
   int32_t* flags;          /* rows_pad / 256 */
@@ -429,7 +429,7 @@ int meep2b_linear_ce_backward(const meep2b_linear_ce* a, void* stream);
  * m_e the mean of p_e, loss = experts * sum_e f_e m_e, and its gradient of the logits (the choice carries none). The
  * choice is `index` (tokens, top_k) per layer, or the top_k largest logits, the lower expert first where they are
  * equal. logits: per layer (tokens, experts) contiguous, bf16 or f32. A masked token (mask byte 0) is not read; its
- * gradient is zero. At most 128 layers and 1024 experts. */
+ * gradient is zero. At most 128 layers, 1024 experts and 2^27 tokens in all layers. */
 typedef struct meep2b_balance {
   const void* const* logits;    /* host array of `layers` device pointers */
   int32_t layers;
@@ -459,7 +459,7 @@ int meep2b_balance_loss_backward(const meep2b_balance* a, void* stream);
  * stay. q (batch, length, q_heads, dim) and k (batch, length, kv_heads, dim) in bf16 or f32 with unit inner stride;
  * strides of the batch, the token and the head in elements, multiples of 16 bytes. positions (batch, length) int64, or
  * NULL for 0 .. length - 1 in every batch; a position outside the angles makes its turned values NaN. dim a multiple of
- * 16 up to 256, half of 8. Outputs are contiguous. */
+ * 16 up to 256, half of 8; batch * length * (q_heads + kv_heads) below 2^30. Outputs are contiguous. */
 typedef struct meep2b_head_norm {
   const void* q;
   const void* k;

@@ -6,6 +6,7 @@ falls back to another implementation: a missing library or a non-zero status rai
 
 import ctypes
 import os
+import struct
 
 import torch
 
@@ -84,6 +85,14 @@ class HeadNorm(ctypes.Structure):
     ]
 
 
+def packer(cls):
+    """struct.Struct of a ctypes.Structure's fields in order, with the C compiler's padding: its pack(*values) gives the
+    argument's bytes in a tenth of the time that filling the Structure takes (arrays as that many values, NULL as 0)."""
+    codes = {_p: "P", _i64: "q", _i32: "i", _f32: "f"}
+    return struct.Struct("@" + "".join(codes[t] if t in codes else f"{t._length_}{codes[t._type_]}"
+                                       for _, t in cls._fields_))
+
+
 _SIGNATURES = {
     "meep2b_version": (ctypes.c_char_p, []),
     "meep2b_status_string": (ctypes.c_char_p, [ctypes.c_int]),
@@ -120,16 +129,17 @@ _SIGNATURES = {
     "meep2b_grouped_product_f8": (ctypes.c_int, [ctypes.POINTER(ProductF8), _p]),
     "meep2b_swiglu": (ctypes.c_int, [_p, _i64, _i64, _p, _p]),
     "meep2b_swiglu_backward": (ctypes.c_int, [_p, _p, _i64, _i64, _p, _p]),
+    # (the arguments of the next six are packed: packer(Balance), packer(HeadNorm), packer(LinearCE))
     "meep2b_balance_workspace_bytes": (_sz, [_i32]),
-    "meep2b_balance_loss": (ctypes.c_int, [ctypes.POINTER(Balance), _p]),
-    "meep2b_balance_loss_backward": (ctypes.c_int, [ctypes.POINTER(Balance), _p]),
+    "meep2b_balance_loss": (ctypes.c_int, [_p, _p]),
+    "meep2b_balance_loss_backward": (ctypes.c_int, [_p, _p]),
     "meep2b_head_norm_partials": (ctypes.c_int, []),
-    "meep2b_head_norm_rotate": (ctypes.c_int, [ctypes.POINTER(HeadNorm), _p]),
-    "meep2b_head_norm_rotate_backward": (ctypes.c_int, [ctypes.POINTER(HeadNorm), _p]),
+    "meep2b_head_norm_rotate": (ctypes.c_int, [_p, _p]),
+    "meep2b_head_norm_rotate_backward": (ctypes.c_int, [_p, _p]),
     "meep2b_linear_ce_plan": (ctypes.c_int, [_i64, _i64, _i64, ctypes.POINTER(_i64), ctypes.POINTER(_i64),
                                              ctypes.POINTER(_i32)]),
-    "meep2b_linear_ce_forward": (ctypes.c_int, [ctypes.POINTER(LinearCE), _p]),
-    "meep2b_linear_ce_backward": (ctypes.c_int, [ctypes.POINTER(LinearCE), _p]),
+    "meep2b_linear_ce_forward": (ctypes.c_int, [_p, _p]),
+    "meep2b_linear_ce_backward": (ctypes.c_int, [_p, _p]),
 }
 
 _lib = None
@@ -214,11 +224,23 @@ def check(status: int, what: str):
     raise RuntimeError(msg)
 
 
+def once(backward):
+    """A Function's backward that is not differentiable itself. torch's own wrapper is put around it only where a second
+    derivative could be asked for (grad mode is on in the backward pass); it takes as long as a small kernel."""
+    return torch.autograd.function.once_differentiable(backward) if torch.is_grad_enabled() else backward
+
+
 def ptr(t):
     return None if t is None else ctypes.c_void_p(t.data_ptr())
 
 
+# the current stream's handle without building a torch.cuda.Stream, where this torch has it (2 us a call less)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def stream_of(t) -> ctypes.c_void_p:
+    if _raw_stream is not None:
+        return ctypes.c_void_p(_raw_stream(t.get_device()))
     return ctypes.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
 
 

@@ -35,6 +35,16 @@ int bind_stream_device(cudaStream_t stream) {
   return MEEP2B_OK;
 }
 
+int device_sms(int* sms) {
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess ||
+      cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) {
+    cudaGetLastError();
+    return MEEP2B_ERR_LAUNCH;
+  }
+  return MEEP2B_OK;
+}
+
 int launch_status() {
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) {

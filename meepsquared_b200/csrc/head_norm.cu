@@ -6,11 +6,13 @@
 //   u = R^T dy,  dw = sum over rows of u n,  v = u w,  dx = r (v - n mean(v n))
 //
 // Bound by memory: x in and y out (forward), x and dy in and dx out (backward), once each. A head is read by a group
-// of 2 to 32 lanes, each with two 16-byte chunks that turn against each other (i and i + half), so that the rotation
+// of 1 to 32 lanes, each with two 16-byte chunks that turn against each other (i and i + half), so that the rotation
 // needs no exchange between lanes and the norm three or four shuffles. A group takes several heads of one token in a
-// row, which keeps the token's cosines and sines and the head weight in registers. A CTA works on queries or on keys
-// alone, in proportion to their heads. The weights' gradients are summed in registers, joined per CTA, and the CTAs'
-// sums by a second kernel in a fixed order.
+// row, which keeps the token's cosines and sines and the head weight in registers. A thread's heads come through a ring
+// of its own in shared memory by 16-byte asynchronous copies, a few heads ahead: enough in flight for HBM without holding
+// registers, and with no barrier. A CTA works on queries or on keys alone. The forward pass has a group for every run of heads; the
+// backward pass with the weights' gradients has as many CTAs as the SMs hold, in proportion to the queries' and the
+// keys' heads: their sums stay in registers, are joined per CTA, and the CTAs' sums by a second kernel in a fixed order.
 #include "common.cuh"
 #include "host.hpp"
 
@@ -18,7 +20,7 @@ namespace meep2b {
 namespace head_norm {
 
 constexpr int THREADS = 256;
-constexpr int MAX_PARTIALS = 1184;  // CTAs of the backward pass that may leave sums: eight per SM
+constexpr int MAX_PARTIALS = 512;  // CTAs of the backward pass that may leave sums
 
 struct Side {  // the queries or the keys
   const void* x;
@@ -28,12 +30,14 @@ struct Side {  // the queries or the keys
   void* y;             // forward: y; backward: dx (contiguous)
   const void* dy;
   int64_t db, dt, dh;
+  int span;            // heads a group takes in a row
 };
 
 struct Params {
   Side side[2];
   int64_t tokens;      // batch * length
-  int length, dim, half, span;  // span: heads a group takes in a row
+  int length, dim, half;
+  int angle_vec;       // cosine and sine rows start on 16 bytes
   const void* cos;
   const void* sin;
   int64_t ld_cos, ld_sin, angles;
@@ -48,32 +52,45 @@ struct Vec;
 template <>
 struct Vec<__nv_bfloat16> {
   static constexpr int N = 8;
-  static __device__ __forceinline__ void load(const void* p, float (&v)[8]) {
-    const uint4 w = *static_cast<const uint4*>(p);
+  static __device__ __forceinline__ void unpack(uint4 w, float (&v)[8]) {
     v[0] = bf16_lo(w.x), v[1] = bf16_hi(w.x), v[2] = bf16_lo(w.y), v[3] = bf16_hi(w.y);
     v[4] = bf16_lo(w.z), v[5] = bf16_hi(w.z), v[6] = bf16_lo(w.w), v[7] = bf16_hi(w.w);
   }
-  static __device__ __forceinline__ void store(void* p, const float (&v)[8]) {
-    *static_cast<uint4*>(p) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
-                                         pack_bf16x2(v[6], v[7]));
+  static __device__ __forceinline__ uint4 pack(const float (&v)[8]) {
+    return make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
+                      pack_bf16x2(v[6], v[7]));
   }
 };
 template <>
 struct Vec<float> {
   static constexpr int N = 4;
-  static __device__ __forceinline__ void load(const void* p, float (&v)[4]) {
-    const float4 w = *static_cast<const float4*>(p);
-    v[0] = w.x, v[1] = w.y, v[2] = w.z, v[3] = w.w;
+  static __device__ __forceinline__ void unpack(uint4 w, float (&v)[4]) {
+    v[0] = __uint_as_float(w.x), v[1] = __uint_as_float(w.y), v[2] = __uint_as_float(w.z), v[3] = __uint_as_float(w.w);
   }
-  static __device__ __forceinline__ void store(void* p, const float (&v)[4]) {
-    *static_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+  static __device__ __forceinline__ uint4 pack(const float (&v)[4]) {
+    return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
   }
 };
 
-// N values of a cosine or sine row; the rows may start anywhere.
+// N values of a cosine or sine row, which may start anywhere unless vec.
 template <typename A, int N>
-__device__ __forceinline__ void load_angles(const void* base, int64_t at, float (&v)[N]) {
+__device__ __forceinline__ void load_angles(const void* base, int64_t at, bool vec, float (&v)[N]) {
   const A* p = static_cast<const A*>(base) + at;
+  if constexpr (sizeof(A) == 4) {
+    if (vec) {
+#pragma unroll
+      for (int j = 0; j < N; j += 4) {
+        const float4 q = __ldg(reinterpret_cast<const float4*>(p + j));
+        v[j] = q.x, v[j + 1] = q.y, v[j + 2] = q.z, v[j + 3] = q.w;
+      }
+      return;
+    }
+  } else if constexpr (N == 8) {
+    if (vec) {
+      Vec<__nv_bfloat16>::unpack(__ldg(reinterpret_cast<const uint4*>(p)), v);
+      return;
+    }
+  }
 #pragma unroll
   for (int j = 0; j < N; ++j) {
     if constexpr (sizeof(A) == 4) v[j] = p[j];
@@ -81,10 +98,29 @@ __device__ __forceinline__ void load_angles(const void* base, int64_t at, float 
   }
 }
 
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Heads a thread's copies run ahead: 8 KB of shared memory a CTA each forward, 16 KB backward (x and dy).
+template <bool BACKWARD>
+struct Ring {
+  static constexpr int CHUNKS = BACKWARD ? 4 : 2;
+  static constexpr int DEPTH = BACKWARD ? 3 : 4;
+  static constexpr int BYTES = DEPTH * CHUNKS * THREADS * 16;
+};
+
 // T: the heads' type; A: the angles'; G: lanes a head; BACKWARD; DW: the weights' gradients too.
 template <typename T, typename A, int G, bool BACKWARD, bool DW>
-__global__ void __launch_bounds__(THREADS) norm_rotate(const Params p) {
+__global__ void __launch_bounds__(THREADS, BACKWARD ? 2 : 3) norm_rotate(const Params p) {
   constexpr int N = Vec<T>::N;
+  using R = Ring<BACKWARD>;
+  extern __shared__ __align__(16) uint8_t ring[];
   const int kind = blockIdx.x >= p.q_blocks;
   const Side& s = p.side[kind];
   const int blocks = kind ? gridDim.x - p.q_blocks : p.q_blocks;
@@ -96,95 +132,147 @@ __global__ void __launch_bounds__(THREADS) norm_rotate(const Params p) {
   const bool here = lane < p.dim / (2 * N), turns = lane < turned;
   const int c0 = turns ? lane : 2 * turned + 2 * (lane - turned), c1 = turns ? lane + turned : c0 + 1;
   const int o0 = c0 * N, o1 = c1 * N;
-  float w0[N] = {}, w1[N] = {}, dw0[N] = {}, dw1[N] = {};
+  float dw0[N] = {}, dw1[N] = {};
+  uint4 wr0 = make_uint4(0, 0, 0, 0), wr1 = wr0;  // the weight as it is stored: half the registers in bf16
   if (here) {
-    Vec<T>::load(static_cast<const T*>(s.weight) + o0, w0);
-    Vec<T>::load(static_cast<const T*>(s.weight) + o1, w1);
+    wr0 = *reinterpret_cast<const uint4*>(static_cast<const T*>(s.weight) + o0);
+    wr1 = *reinterpret_cast<const uint4*>(static_cast<const T*>(s.weight) + o1);
   }
-  const int spans = (s.heads + p.span - 1) / p.span;
-  const int64_t items = p.tokens * spans;
+  // items fit 31 bits (the entry point's limit on tokens x heads), and a stride more 32
+  const int span = s.span;
+  const uint32_t spans = (s.heads + span - 1) / span;
+  const uint32_t items = static_cast<uint32_t>(p.tokens) * spans;
   const float inv_dim = 1.0f / static_cast<float>(p.dim);
-  const int64_t stride = static_cast<int64_t>(blocks) * GROUPS;
+  const uint32_t stride = static_cast<uint32_t>(blocks) * GROUPS;
   // every group of a warp makes the same number of rounds, so that the shuffles below have all their lanes
-  const int64_t first = static_cast<int64_t>(block) * GROUPS + group;
-  const int64_t warp_first = static_cast<int64_t>(block) * GROUPS + (threadIdx.x & ~31) / G;
-  for (int64_t base = warp_first, item = first; base < items; base += stride, item += stride) {
-    const bool live = item < items;
-    const int64_t t = live ? item / spans : 0;
-    const int h0 = live ? static_cast<int>(item - t * spans) * p.span : 0;
-    const int64_t b = t / p.length;
-    const int l = static_cast<int>(t - b * p.length);
-    float cs[N], sn[N];
-#pragma unroll
-    for (int j = 0; j < N; ++j) cs[j] = 1.f, sn[j] = 0.f;
-    if (live && turns) {
-      const int64_t pos = p.positions ? p.positions[t] : l;
-      if (pos >= 0 && pos < p.angles) {
-        load_angles<A, N>(p.cos, pos * p.ld_cos + o0, cs);
-        load_angles<A, N>(p.sin, pos * p.ld_sin + o0, sn);
-      } else {  // a position without angles
-#pragma unroll
-        for (int j = 0; j < N; ++j) cs[j] = sn[j] = __int_as_float(0x7fc00000);
+  const uint32_t first = static_cast<uint32_t>(block) * GROUPS + group;
+  const uint32_t warp_first = static_cast<uint32_t>(block) * GROUPS + (threadIdx.x & ~31) / G;
+  const int rounds = warp_first < items ? static_cast<int>((items - 1 - warp_first) / stride) + 1 : 0;
+  const int steps = rounds * span;
+
+  // the copies' side: step after step, a head each
+  uint32_t c_item = first;
+  int c_head = 0, c_left = 0, c_slot = 0;
+  const T *c_x = nullptr, *c_dy = nullptr;
+  const uint32_t mine = smem_u32(ring) + threadIdx.x * 16u;
+  auto copy_next = [&]() {
+    if (c_left == 0) {  // the next item
+      const bool live = c_item < items;
+      const uint32_t t = live ? c_item / spans : 0;
+      const uint32_t b = t / static_cast<uint32_t>(p.length), l = t - b * static_cast<uint32_t>(p.length);
+      c_head = live ? static_cast<int>(c_item - t * spans) * span : s.heads;
+      c_x = static_cast<const T*>(s.x) + b * s.sb + l * s.st + c_head * s.sh;
+      if (BACKWARD) c_dy = static_cast<const T*>(s.dy) + b * s.db + l * s.dt + c_head * s.dh;
+      c_left = span;
+      c_item += stride;
+    }
+    if (here && c_head < s.heads) {
+      const uint32_t at = mine + c_slot * (R::CHUNKS * THREADS * 16u);
+      copy16(at, c_x + o0);
+      copy16(at + THREADS * 16u, c_x + o1);
+      if (BACKWARD) {
+        copy16(at + 2 * THREADS * 16u, c_dy + o0);
+        copy16(at + 3 * THREADS * 16u, c_dy + o1);
       }
     }
-    const T* x = static_cast<const T*>(s.x) + b * s.sb + l * s.st;
-    const T* dy = BACKWARD ? static_cast<const T*>(s.dy) + b * s.db + l * s.dt : nullptr;
-    T* y = static_cast<T*>(s.y) + t * s.heads * p.dim;
-#pragma unroll 2
-    for (int i = 0; i < p.span; ++i) {
-      const int h = h0 + i;
-      const bool on = live && here && h < s.heads;
-      float a[N] = {}, c[N] = {};
-      if (on) {
-        Vec<T>::load(x + h * s.sh + o0, a);
-        Vec<T>::load(x + h * s.sh + o1, c);
-      }
-      float u0[N] = {}, u1[N] = {};
-      if (BACKWARD && on) {
-        Vec<T>::load(dy + h * s.dh + o0, u0);
-        Vec<T>::load(dy + h * s.dh + o1, u1);
-      }
-      float sq = 0.f;
+    ++c_head, --c_left;
+    c_x += s.sh;
+    if (BACKWARD) c_dy += s.dh;
+    c_slot = c_slot + 1 == R::DEPTH ? 0 : c_slot + 1;
+  };
 #pragma unroll
-      for (int j = 0; j < N; ++j) sq = fmaf(a[j], a[j], fmaf(c[j], c[j], sq));
+  for (int i = 0; i < R::DEPTH - 1; ++i) {
+    if (i < steps) copy_next();
+    copies_commit();
+  }
+
+  float cs[N], sn[N];
+  T* y = nullptr;
+  uint32_t item = first;
+  int head = 0, left = 0, slot = 0;
+  for (int step = 0; step < steps; ++step) {
+    if (left == 0) {  // the next item: its angles
+      const bool live = item < items;
+      const uint32_t t = live ? item / spans : 0;
+      head = live ? static_cast<int>(item - t * spans) * span : s.heads;
+      y = static_cast<T*>(s.y) + (static_cast<int64_t>(t) * s.heads + head) * p.dim;
 #pragma unroll
-      for (int off = G / 2; off > 0; off >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, off);
-      const float r = rsqrtf(fmaf(sq, inv_dim, p.eps));
-      if (!BACKWARD) {
+      for (int j = 0; j < N; ++j) cs[j] = 1.f, sn[j] = 0.f;
+      if (live && turns) {
+        const int64_t pos = p.positions ? p.positions[t] : t % static_cast<uint32_t>(p.length);
+        if (pos >= 0 && pos < p.angles) {
+          load_angles<A, N>(p.cos, pos * p.ld_cos + o0, p.angle_vec, cs);
+          load_angles<A, N>(p.sin, pos * p.ld_sin + o0, p.angle_vec, sn);
+        } else {  // a position without angles
 #pragma unroll
-        for (int j = 0; j < N; ++j) {
-          const float e = a[j] * r * w0[j], f = c[j] * r * w1[j];
-          a[j] = turns ? e * cs[j] - f * sn[j] : e;
-          c[j] = turns ? f * cs[j] + e * sn[j] : f;
-        }
-      } else {
-        float mean = 0.f;
-#pragma unroll
-        for (int j = 0; j < N; ++j) {
-          a[j] *= r, c[j] *= r;
-          const float e = turns ? u0[j] * cs[j] + u1[j] * sn[j] : u0[j];
-          const float f = turns ? u1[j] * cs[j] - u0[j] * sn[j] : u1[j];
-          if (DW) dw0[j] = fmaf(e, a[j], dw0[j]), dw1[j] = fmaf(f, c[j], dw1[j]);
-          u0[j] = e * w0[j], u1[j] = f * w1[j];
-          mean = fmaf(u0[j], a[j], fmaf(u1[j], c[j], mean));
-        }
-#pragma unroll
-        for (int off = G / 2; off > 0; off >>= 1) mean += __shfl_xor_sync(0xffffffffu, mean, off);
-        mean *= inv_dim;
-#pragma unroll
-        for (int j = 0; j < N; ++j) {
-          a[j] = r * (u0[j] - a[j] * mean);
-          c[j] = r * (u1[j] - c[j] * mean);
+          for (int j = 0; j < N; ++j) cs[j] = sn[j] = __int_as_float(0x7fc00000);
         }
       }
-      if (on) {
-        Vec<T>::store(y + h * p.dim + o0, a);
-        Vec<T>::store(y + h * p.dim + o1, c);
+      left = span;
+      item += stride;
+    }
+    if (step + R::DEPTH - 1 < steps) copy_next();
+    copies_commit();
+    copies_wait<R::DEPTH - 1>();
+    const bool on = here && head < s.heads;
+    uint4 rx0 = make_uint4(0, 0, 0, 0), rx1 = rx0, rd0 = rx0, rd1 = rx0;
+    if (on) {
+      const uint4* at = reinterpret_cast<const uint4*>(ring) + slot * (R::CHUNKS * THREADS) + threadIdx.x;
+      rx0 = at[0], rx1 = at[THREADS];
+      if (BACKWARD) rd0 = at[2 * THREADS], rd1 = at[3 * THREADS];
+    }
+    float a[N], c[N], w0[N], w1[N];
+    Vec<T>::unpack(rx0, a), Vec<T>::unpack(rx1, c);
+    float sq = 0.f;
+#pragma unroll
+    for (int j = 0; j < N; ++j) sq = fmaf(a[j], a[j], fmaf(c[j], c[j], sq));
+#pragma unroll
+    for (int off = G / 2; off > 0; off >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, off);
+    const float r = rsqrtf(fmaf(sq, inv_dim, p.eps));
+    Vec<T>::unpack(wr0, w0), Vec<T>::unpack(wr1, w1);
+    if (!BACKWARD) {
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const float e = a[j] * r * w0[j], f = c[j] * r * w1[j];
+        a[j] = turns ? e * cs[j] - f * sn[j] : e;
+        c[j] = turns ? f * cs[j] + e * sn[j] : f;
+      }
+    } else {
+      float u0[N], u1[N];
+      Vec<T>::unpack(rd0, u0), Vec<T>::unpack(rd1, u1);
+      float mean = 0.f;
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        a[j] *= r, c[j] *= r;
+        const float e = turns ? u0[j] * cs[j] + u1[j] * sn[j] : u0[j];
+        const float f = turns ? u1[j] * cs[j] - u0[j] * sn[j] : u1[j];
+        if (DW) {
+          if (on) dw0[j] = fmaf(e, a[j], dw0[j]), dw1[j] = fmaf(f, c[j], dw1[j]);
+        }
+        u0[j] = e * w0[j], u1[j] = f * w1[j];
+        mean = fmaf(u0[j], a[j], fmaf(u1[j], c[j], mean));
+      }
+#pragma unroll
+      for (int off = G / 2; off > 0; off >>= 1) mean += __shfl_xor_sync(0xffffffffu, mean, off);
+      mean *= inv_dim;
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        a[j] = r * (u0[j] - a[j] * mean);
+        c[j] = r * (u1[j] - c[j] * mean);
       }
     }
+    if (on) {
+      *reinterpret_cast<uint4*>(y + o0) = Vec<T>::pack(a);
+      *reinterpret_cast<uint4*>(y + o1) = Vec<T>::pack(c);
+    }
+    ++head, --left;
+    y += p.dim;
+    slot = slot + 1 == R::DEPTH ? 0 : slot + 1;
   }
   if (DW) {  // the CTA's sum, group after group
-    extern __shared__ float sums[];  // (GROUPS, dim)
+    float* sums = reinterpret_cast<float*>(ring);  // (GROUPS, dim): at most 16 KB
+    copies_wait<0>();
+    __syncthreads();
     if (here) {
 #pragma unroll
       for (int j = 0; j < N; ++j) {
@@ -195,6 +283,7 @@ __global__ void __launch_bounds__(THREADS) norm_rotate(const Params p) {
     __syncthreads();
     for (int d = threadIdx.x; d < p.dim; d += THREADS) {
       float t = 0.f;
+#pragma unroll 8
       for (int g = 0; g < GROUPS; ++g) t += sums[g * p.dim + d];
       p.partial[static_cast<int64_t>(blockIdx.x) * p.dim + d] = t;
     }
@@ -212,6 +301,7 @@ __global__ void __launch_bounds__(1024) join_weight(const float* __restrict__ pa
   const int b0 = blockIdx.y ? q_blocks : 0, b1 = blockIdx.y ? blocks : q_blocks;
   float t = 0.f;
   if (d < dim)
+#pragma unroll 8
     for (int b = b0 + y; b < b1; b += 32) t += partial[static_cast<int64_t>(b) * dim + d];
   sums[y][x] = t;
   __syncthreads();
@@ -225,12 +315,12 @@ __global__ void __launch_bounds__(1024) join_weight(const float* __restrict__ pa
 }
 
 template <typename T, typename A, bool BACKWARD, bool DW>
-static void launch(const Params& p, int blocks, cudaStream_t s) {
+static void launch(const Params& p, unsigned blocks, cudaStream_t s) {
   const int slots = p.dim / (2 * Vec<T>::N);  // lanes a head needs
 #define MEEP2B_HEADS(G)                                                                                      \
-  norm_rotate<T, A, G, BACKWARD, DW>                                                                          \
-      <<<blocks, THREADS, DW ? static_cast<size_t>(THREADS / G) * p.dim * sizeof(float) : 0, s>>>(p)
-  if (slots <= 2) MEEP2B_HEADS(2);
+  norm_rotate<T, A, G, BACKWARD, DW><<<blocks, THREADS, Ring<BACKWARD>::BYTES, s>>>(p)
+  if (slots <= 1) MEEP2B_HEADS(1);
+  else if (slots <= 2) MEEP2B_HEADS(2);
   else if (slots <= 4) MEEP2B_HEADS(4);
   else if (slots <= 8) MEEP2B_HEADS(8);
   else if (slots <= 16) MEEP2B_HEADS(16);
@@ -239,7 +329,7 @@ static void launch(const Params& p, int blocks, cudaStream_t s) {
 }
 
 template <bool BACKWARD, bool DW>
-static void launch_types(const Params& p, int dtype, int angle_dtype, int blocks, cudaStream_t s) {
+static void launch_types(const Params& p, int dtype, int angle_dtype, unsigned blocks, cudaStream_t s) {
   if (dtype == MEEP2B_BF16) {
     if (angle_dtype == MEEP2B_BF16) launch<__nv_bfloat16, __nv_bfloat16, BACKWARD, DW>(p, blocks, s);
     else launch<__nv_bfloat16, float, BACKWARD, DW>(p, blocks, s);
@@ -249,35 +339,34 @@ static void launch_types(const Params& p, int dtype, int angle_dtype, int blocks
   }
 }
 
-// How the heads of a token are taken: up to 8 in a row, fewer while that leaves groups without work. blocks: enough
-// CTAs for every item, or what the SMs hold at once.
-static int shape(Params& p, int lanes, int sms, int most_blocks) {
+// How the heads of a token are taken: up to 8 in a row, fewer while that leaves groups without work, in runs of about
+// one length. Returns the CTAs: one for every GROUPS items, or `most` of them in proportion to the queries' and the
+// keys' heads.
+static int64_t shape(Params& p, int lanes, int sms, int64_t most) {
   const int groups = THREADS / lanes;
   const int64_t heads = p.side[0].heads + p.side[1].heads;
-  const int64_t wanted = static_cast<int64_t>(sms) * 8 * groups;  // groups that keep the memory busy
-  p.span = 8;
-  while (p.span > 1 && p.tokens * heads / p.span < wanted) p.span /= 2;
-  int64_t items = 0, q_items = 0;
+  const int64_t wanted = static_cast<int64_t>(sms) * 3 * groups;  // groups the SMs hold at once
+  int span = 8;
+  while (span > 1 && p.tokens * heads / span < wanted) span /= 2;
+  int64_t blocks[2];
   for (int i = 0; i < 2; ++i) {
-    const int64_t n = p.tokens * ((p.side[i].heads + p.span - 1) / p.span);
-    items += n;
-    if (i == 0) q_items = n;
+    const int runs = (p.side[i].heads + span - 1) / span;
+    p.side[i].span = (p.side[i].heads + runs - 1) / runs;
+    const int64_t items = p.tokens * ((p.side[i].heads + p.side[i].span - 1) / p.side[i].span);
+    blocks[i] = (items + groups - 1) / groups;
   }
-  int64_t blocks = (q_items + groups - 1) / groups + (items - q_items + groups - 1) / groups;
-  if (blocks <= most_blocks) {
-    p.q_blocks = static_cast<int>((q_items + groups - 1) / groups);
-    return static_cast<int>(blocks);
+  if (blocks[0] + blocks[1] > most) {
+    blocks[0] = most * p.side[0].heads / heads;
+    blocks[0] = blocks[0] < 1 ? 1 : (blocks[0] > most - 1 ? most - 1 : blocks[0]);
+    blocks[1] = most - blocks[0];
   }
-  blocks = most_blocks;
-  int q = static_cast<int>(blocks * q_items / items);
-  q = q < 1 ? 1 : (q > blocks - 1 ? static_cast<int>(blocks) - 1 : q);
-  p.q_blocks = q;
-  return static_cast<int>(blocks);
+  p.q_blocks = static_cast<int>(blocks[0]);
+  return blocks[0] + blocks[1];
 }
 
 static int lanes_of(int dim, int dtype) {
   const int slots = dim / (dtype == MEEP2B_BF16 ? 16 : 8);
-  int g = 2;
+  int g = 1;
   while (g < slots) g *= 2;
   return g;
 }
@@ -307,13 +396,16 @@ int head_norm_params(const meep2b_head_norm* a, bool backward, head_norm::Params
     return MEEP2B_ERR_ALIGN;
   head_norm::Params p = {};
   p.side[0] = {a->q, a->q_stride[0], a->q_stride[1], a->q_stride[2], a->q_heads, a->q_weight, a->q_out,
-               a->dq_out, a->dq_out_stride[0], a->dq_out_stride[1], a->dq_out_stride[2]};
+               a->dq_out, a->dq_out_stride[0], a->dq_out_stride[1], a->dq_out_stride[2], 1};
   p.side[1] = {a->k, a->k_stride[0], a->k_stride[1], a->k_stride[2], a->kv_heads, a->k_weight, a->k_out,
-               a->dk_out, a->dk_out_stride[0], a->dk_out_stride[1], a->dk_out_stride[2]};
+               a->dk_out, a->dk_out_stride[0], a->dk_out_stride[1], a->dk_out_stride[2], 1};
   p.tokens = a->batch * a->length, p.length = static_cast<int>(a->length);
   p.dim = a->dim, p.half = a->half;
   p.cos = a->cos, p.sin = a->sin, p.ld_cos = a->ld_cos, p.ld_sin = a->ld_sin, p.angles = a->angles;
   p.positions = a->positions, p.eps = a->eps;
+  const int64_t angle_vec = a->angle_dtype == MEEP2B_BF16 ? 8 : 4;
+  p.angle_vec = aligned16(a->cos) && aligned16(a->sin) && a->ld_cos % angle_vec == 0 && a->ld_sin % angle_vec == 0;
+  if (a->batch > INT32_MAX || p.tokens > (INT32_MAX >> 1) / (a->q_heads + a->kv_heads)) return MEEP2B_ERR_SHAPE;
   *out = p;
   return MEEP2B_OK;
 }
@@ -330,8 +422,10 @@ int meep2b_head_norm_rotate(const meep2b_head_norm* a, void* stream) {
   cudaStream_t s = as_stream(stream);
   MEEP2B_TRY(bind_stream_device(s));
   if (p.tokens == 0) return MEEP2B_OK;
-  const int blocks = head_norm::shape(p, head_norm::lanes_of(p.dim, a->dtype), 148, 148 * 8);
-  head_norm::launch_types<false, false>(p, a->dtype, a->angle_dtype, blocks, s);
+  int sms = 0;
+  MEEP2B_TRY(device_sms(&sms));
+  const int64_t blocks = head_norm::shape(p, head_norm::lanes_of(p.dim, a->dtype), sms, INT32_MAX);
+  head_norm::launch_types<false, false>(p, a->dtype, a->angle_dtype, static_cast<unsigned>(blocks), s);
   return launch_status();
 }
 
@@ -345,7 +439,10 @@ int meep2b_head_norm_rotate_backward(const meep2b_head_norm* a, void* stream) {
   p.partial = a->partial;
   int blocks = 0;
   if (p.tokens > 0) {
-    blocks = head_norm::shape(p, head_norm::lanes_of(p.dim, a->dtype), 148, head_norm::MAX_PARTIALS);
+    int sms = 0;
+    MEEP2B_TRY(device_sms(&sms));
+    const int64_t most = !dw ? INT32_MAX : (2 * sms < head_norm::MAX_PARTIALS ? 2 * sms : head_norm::MAX_PARTIALS);
+    blocks = static_cast<int>(head_norm::shape(p, head_norm::lanes_of(p.dim, a->dtype), sms, most));
     if (dw) head_norm::launch_types<true, true>(p, a->dtype, a->angle_dtype, blocks, s);
     else head_norm::launch_types<true, false>(p, a->dtype, a->angle_dtype, blocks, s);
     MEEP2B_TRY(launch_status());

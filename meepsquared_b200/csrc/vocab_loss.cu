@@ -77,17 +77,19 @@ struct Params {
   int vocab, hidden;
   int v0, piece_tiles;     // the piece: its first column and its column tiles
   int k_total;             // depth of the product, in elements (kAcc: the piece's columns; kWeight: live rows)
-  int planes;              // kAcc: the most parts the depth may be split into, each summed in a plane of its own
+  int planes, depth;       // kAcc: the most parts the depth may be split into, each summed in a plane of its own, and
+                           // a whole piece's depth, which decides how many are used
   int first;               // kAcc: the first piece (stores)
 };
 
-// Into how many parts the depth of a product of `units` tiles is split on `pairs` CTA pairs: the number whose last
-// round of units leaves the least idle, each part costing about 1% of a round (its plane written and read again).
-__host__ __device__ inline int depth_parts(int units, int pairs, int most) {
+// Into how many parts the depth k of a product of `units` tiles is split on `pairs` CTA pairs: the number whose last
+// round of units leaves the least idle, against the plane that each part costs (written, and read at the end: 8 bytes a
+// value at 6.5 TB/s, where a round of 74 units of depth k takes k 6.5 ns).
+__host__ __device__ inline int depth_parts(int units, int pairs, int most, int k) {
   int best = 1;
   float best_cost = 1e30f;
   for (int s = 1; s <= most; ++s) {
-    const float cost = static_cast<float>((units * s + pairs - 1) / pairs) / s + 0.01f * s;
+    const float cost = static_cast<float>((units * s + pairs - 1) / pairs) / s + 12.5f * units * s / k;
     if (cost < best_cost) best_cost = cost, best = s;
   }
   return best;
@@ -119,7 +121,7 @@ __device__ __forceinline__ Units units_of(const Params& p, int pairs) {
     w.kblocks = (live + BK - 1) / BK;
   } else if (MODE == kAcc) {
     w.mt = row_tiles, w.nt = (p.hidden + TILE - 1) / TILE;
-    w.parts = depth_parts(w.mt * w.nt, pairs, p.planes);
+    w.parts = depth_parts(w.mt * w.nt, pairs, p.planes, p.depth);
     w.kblocks = (p.k_total + BK - 1) / BK;
   } else {
     w.mt = row_tiles, w.nt = p.piece_tiles, w.parts = 1;
@@ -169,6 +171,9 @@ __device__ __forceinline__ float row_upstream(const float* upstream, int per_tok
   const float g = upstream[per_token ? token : 0];
   return mean ? g / static_cast<float>(max(live, 1)) : g;
 }
+
+// The gradient of the target's own logit, g (p - 1).
+__device__ __forceinline__ float target_gradient(float miss, float g) { return __fmul_rn(-miss, g); }
 
 // One unit's epilogue for one warp: 32 rows (a lane each) and 128 columns, 32 at a time.
 template <int MODE>
@@ -227,13 +232,13 @@ __device__ __forceinline__ void epilogue(const Params& p, const CUtensorMap* out
           far = here != here ? here : (far != far ? far : hi + log2f(1.0f + exp2f(lo - hi)));
         }
       }
-      if (MODE == kGrad) {
+      if (MODE == kGrad) {  // (rows past the last live one are zero: the head's gradient sums over them)
 #pragma unroll
-        for (int j = 0; j < 32; ++j) e[j] *= g;
+        for (int j = 0; j < 32; ++j) e[j] = row < live ? e[j] * g : 0.f;
         if (target >= vcol && target < vcol + 32) {
 #pragma unroll
           for (int j = 0; j < 32; ++j)
-            if (vcol + j == target) e[j] = -miss * g;
+            if (vcol + j == target) e[j] = target_gradient(miss, g);
         }
       }
       if (MODE != kStats) {
@@ -298,8 +303,8 @@ __device__ __forceinline__ void epilogue(const Params& p, const CUtensorMap* out
 
 template <int MODE, bool REDO>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
-    vocab_product(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb,
-                  const __grid_constant__ CUtensorMap tout, const Params p) {
+    vocab_product(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap ta32,
+                  const __grid_constant__ CUtensorMap tb, const __grid_constant__ CUtensorMap tout, const Params p) {
   constexpr bool A_MN = MODE == kWeight;
   constexpr bool B_MN = MODE == kWeight || MODE == kAcc;
   if (REDO && p.state[kRedo] == 0) return;
@@ -357,17 +362,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         if (REDO && p.flags[m] == 0) continue;
         const int a0 = m * TILE + 128 * static_cast<int>(rank), b0 = n * TILE + 128 * static_cast<int>(rank);
         const int k1 = w.k_begin(part + 1);
+        // of a row tile that is not full only the runs of 32 rows that hold live ones are loaded; what stands in the
+        // others' places meets nothing but its own rows of the accumulator
+        const int have = A_MN ? TILE : live - m * TILE;
+        const int runs0 = min(4, max(0, (have + 31) / 32)), runs1 = min(4, max(0, (have - 128 + 31) / 32));
+        const int runs = rank == 0 ? runs0 : runs1;
+        const uint32_t bytes = 2 * OPERAND_BYTES + static_cast<uint32_t>(runs0 + runs1) * (OPERAND_BYTES / 4);
         for (int kb = w.k_begin(part); kb < k1; ++kb) {
           if (!mbar_wait(bar_empty(stage), phase ^ 1)) { ok = false; break; }
           const uint32_t fb = map_to_rank(bar_full(stage), 0);
           const uint32_t a_dst = sbase + stage * STAGE_BYTES, b_dst = a_dst + OPERAND_BYTES;
           const int k0 = kb * BK;
-          if (rank == 0) mbar_arrive_expect_tx(bar_full(stage), 2 * STAGE_BYTES);
+          if (rank == 0) mbar_arrive_expect_tx(bar_full(stage), bytes);
           if (A_MN) {
             tma_load_2d_pair(a_dst, &ta, fb, a0, k0);
             tma_load_2d_pair(a_dst + 8192, &ta, fb, a0 + 64, k0);
-          } else {
+          } else if (runs == 4) {
             tma_load_2d_pair(a_dst, &ta, fb, k0, a0);
+          } else {
+            for (int i = 0; i < runs; ++i) tma_load_2d_pair(a_dst + i * (OPERAND_BYTES / 4), &ta32, fb, k0, a0 + 32 * i);
           }
           if (B_MN) {
             const int kr = MODE == kAcc ? p.v0 + k0 : k0;
@@ -454,6 +467,30 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
 
 // ---------------------------------------------------------------------------------------------------- rows
 
+// How many of a CTA's threads' earlier threads' tokens have a target, and the CTA's total (in *total): each thread gives
+// its own number. words: one int a warp.
+template <int WARPS>
+__device__ __forceinline__ int scan_before(int mine, int* words, int* total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int incl = mine;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, incl, off);
+    if (lane >= off) incl += v;
+  }
+  if (lane == 31) words[warp] = incl;
+  __syncthreads();
+  int before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < WARPS; ++w) {
+    const int v = words[w];
+    if (w < warp) before += v;
+    all += v;
+  }
+  *total = all;
+  return before + incl - mine;
+}
+
 // The tokens with a target, in order: source (live row -> token), slot (token -> live row, or -1), their number; the
 // losses of the ignored tokens (zero) and the state words of this call. One CTA, each thread a run of tokens: the
 // ids are 8 bytes a token and the block's scan is one, so 16,384 tokens take a few microseconds.
@@ -462,31 +499,13 @@ __global__ void __launch_bounds__(1024) vocab_scan(const int64_t* __restrict__ t
                                                   int32_t* __restrict__ slot, int32_t* __restrict__ state,
                                                   int32_t* __restrict__ flags, int row_tiles,
                                                   float* __restrict__ token_loss) {
-  __shared__ int warp_sum[32];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  __shared__ int words[32];
   const int64_t per = (tokens + 1023) / 1024;
   const int64_t t0 = min(tokens, per * threadIdx.x), t1 = min(tokens, t0 + per);
   int mine = 0;
   for (int64_t t = t0; t < t1; ++t) mine += targets[t] != ignore;
-  int incl = mine;
-#pragma unroll
-  for (int off = 1; off < 32; off <<= 1) {
-    const int v = __shfl_up_sync(0xffffffffu, incl, off);
-    if (lane >= off) incl += v;
-  }
-  if (lane == 31) warp_sum[warp] = incl;
-  __syncthreads();
-  if (warp == 0) {
-    int v = warp_sum[lane];
-#pragma unroll
-    for (int off = 1; off < 32; off <<= 1) {
-      const int o = __shfl_up_sync(0xffffffffu, v, off);
-      if (lane >= off) v += o;
-    }
-    warp_sum[lane] = v;
-  }
-  __syncthreads();
-  int at = incl - mine + (warp ? warp_sum[warp - 1] : 0);
+  int total;
+  int at = scan_before<32>(mine, words, &total);
   for (int64_t t = t0; t < t1; ++t) {
     const bool is = targets[t] != ignore;
     slot[t] = is ? at : -1;
@@ -494,21 +513,61 @@ __global__ void __launch_bounds__(1024) vocab_scan(const int64_t* __restrict__ t
     if (!is && token_loss != nullptr) token_loss[t] = 0.f;
   }
   for (int i = threadIdx.x; i < row_tiles; i += 1024) flags[i] = 0;
-  if (threadIdx.x < kStateInts) state[threadIdx.x] = threadIdx.x == kLive ? warp_sum[31] : 0;
+  if (threadIdx.x < kStateInts) state[threadIdx.x] = threadIdx.x == kLive ? total : 0;
 }
 
 // Each live row copied to the front of `compact`, its target and its target's logit (a float32 dot product): a warp
 // per row. The rows from the last live one to the end of its 256-row tile are zero (the head's gradient sums over
 // them). A target outside the vocabulary makes the row's reference, and with it its loss and its gradient, NaN.
+// SCAN: without vocab_scan, whose work each CTA then does for itself, the first one writing it down: a launch less,
+// which counts where there are few tokens (up to kScanned: 32 KB of ids a CTA, from L2).
+constexpr int kScanned = 4096;
+template <bool SCAN>
 __global__ void __launch_bounds__(256) vocab_gather(const __nv_bfloat16* __restrict__ hidden, int64_t ld_hidden,
                                                    const __nv_bfloat16* __restrict__ weight, int64_t ld_weight,
-                                                   const int64_t* __restrict__ targets, int vocab, int width,
-                                                   const int32_t* __restrict__ state,
-                                                   const int32_t* __restrict__ source, __nv_bfloat16* __restrict__ compact,
-                                                   int32_t* __restrict__ target, Rows rows) {
+                                                   const int64_t* __restrict__ targets, int tokens, int64_t ignore,
+                                                   int vocab, int width, int32_t* __restrict__ state,
+                                                   int32_t* __restrict__ flags, int row_tiles,
+                                                   int32_t* __restrict__ source, int32_t* __restrict__ slot,
+                                                   float* __restrict__ token_loss,
+                                                   __nv_bfloat16* __restrict__ compact, int32_t* __restrict__ target,
+                                                   Rows rows) {
   const int lane = threadIdx.x & 31;
   const int row = blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int live = state[kLive];
+  int live, from = 0;
+  if (SCAN) {
+    __shared__ int words[8], mine_rows[8];
+    const int per = (tokens + 255) / 256;
+    const int t0 = min(tokens, per * static_cast<int>(threadIdx.x)), t1 = min(tokens, t0 + per);
+    int mine = 0;
+    uint32_t has = 0;  // per <= 16
+    for (int t = t0; t < t1; ++t) {
+      const bool is = targets[t] != ignore;
+      has |= static_cast<uint32_t>(is) << (t - t0);
+      mine += is;
+    }
+    int at = scan_before<8>(mine, words, &live);
+    const bool writes = blockIdx.x == 0;
+    for (int t = t0; t < t1; ++t) {
+      const bool is = (has >> (t - t0)) & 1u;
+      if (is && at / 8 == static_cast<int>(blockIdx.x)) mine_rows[at % 8] = t;
+      if (writes) {
+        slot[t] = is ? at : -1;
+        if (is) source[at] = t;
+        if (!is && token_loss != nullptr) token_loss[t] = 0.f;
+      }
+      at += is;
+    }
+    if (writes) {
+      if (threadIdx.x < row_tiles) flags[threadIdx.x] = 0;
+      if (threadIdx.x < kStateInts) state[threadIdx.x] = threadIdx.x == kLive ? live : 0;
+    }
+    __syncthreads();
+    if (row < live) from = mine_rows[threadIdx.x >> 5];
+  } else {
+    live = state[kLive];
+    if (row < live) from = source[row];
+  }
   if (row >= (live + TILE - 1) / TILE * TILE) return;
   uint4* to = reinterpret_cast<uint4*>(compact + static_cast<int64_t>(row) * width);
   const int vecs = width / 8;
@@ -520,12 +579,13 @@ __global__ void __launch_bounds__(256) vocab_gather(const __nv_bfloat16* __restr
     }
     return;
   }
-  const int64_t t = source[row];
+  const int64_t t = from;
   const int64_t y = targets[t];
   const bool inside = y >= 0 && y < vocab;
   const uint4* h = reinterpret_cast<const uint4*>(hidden + t * ld_hidden);
   const uint4* wr = reinterpret_cast<const uint4*>(weight + (inside ? y : 0) * ld_weight);
   float dot = 0.f;
+#pragma unroll 4
   for (int i = lane; i < vecs; i += 32) {
     const uint4 a = h[i], b = wr[i];
     to[i] = a;
@@ -559,13 +619,21 @@ __global__ void __launch_bounds__(1024) vocab_join(const float* __restrict__ par
   const int row = blockIdx.x * 32 + x;
   if (row < live) {
     float sum = 0.f, far = -INFINITY;
-    for (int s = y; s < slots; s += 32) {
-      const float v = part[static_cast<int64_t>(s) * rows_pad + row];
-      if (v < 0.f) {
-        const float hi = fmaxf(far, -v), lo = fminf(far, -v);
-        far = hi + log2f(1.0f + exp2f(lo - hi));
-      } else {
-        sum += v;  // (a NaN stays one)
+    for (int s0 = y; s0 < slots; s0 += 32 * 16) {
+      float v[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int s = s0 + 32 * i;
+        v[i] = s < slots ? part[static_cast<int64_t>(s) * rows_pad + row] : 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        if (v[i] < 0.f) {
+          const float hi = fmaxf(far, -v[i]), lo = fminf(far, -v[i]);
+          far = hi + log2f(1.0f + exp2f(lo - hi));
+        } else {
+          sum += v[i];  // (a NaN stays one)
+        }
       }
     }
     sums[y][x] = sum, fars[y][x] = far;
@@ -627,15 +695,16 @@ __global__ void __launch_bounds__(1024) vocab_join(const float* __restrict__ par
   }
 }
 
-// dh of every token from its row's planes: g (scale sum_planes - miss W_y), or the planes' sum alone where the
-// product was over the gradient itself (weight == nullptr); zero for ignored tokens. A warp per token.
-__global__ void __launch_bounds__(256) vocab_finish(const float* __restrict__ acc, int pairs, int planes,
+// dh of every token from its row's planes, zero for ignored tokens. From the forward pass's q: g (scale sum_planes -
+// miss W_y). From the product over g (p - [v = y]) in bf16 (`rounded`): the sum, and what the rounding of the target's
+// value took times W_y, which is the largest rounding of a row by far. A warp per token.
+__global__ void __launch_bounds__(256) vocab_finish(const float* __restrict__ acc, int pairs, int planes, int depth,
                                                    int64_t rows_pad, int width, int64_t tokens,
                                                    const int32_t* __restrict__ state, const int32_t* __restrict__ slot,
                                                    const int32_t* __restrict__ target, Rows rows,
                                                    const __nv_bfloat16* __restrict__ weight, int64_t ld_weight,
                                                    const float* __restrict__ upstream, int per_token, int mean,
-                                                   __nv_bfloat16* __restrict__ d_hidden) {
+                                                   bool rounded, __nv_bfloat16* __restrict__ d_hidden) {
   const int lane = threadIdx.x & 31;
   const int64_t t = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
   if (t >= tokens) return;
@@ -647,15 +716,13 @@ __global__ void __launch_bounds__(256) vocab_finish(const float* __restrict__ ac
     return;
   }
   const int live = state[kLive];
-  const int parts = depth_parts((live + TILE - 1) / TILE * ((width + TILE - 1) / TILE), pairs, planes);
-  float a = 1.f, b = 0.f;
-  const uint4* wr = nullptr;
-  if (weight != nullptr) {
-    const float g = row_upstream(upstream, per_token, mean, static_cast<int>(t), live);
-    a = g * rows.scale[row], b = g * rows.miss[row];
-    const int y = target[row];
-    wr = reinterpret_cast<const uint4*>(weight + static_cast<int64_t>(y < 0 ? 0 : y) * ld_weight);
-  }
+  const int parts = depth_parts((live + TILE - 1) / TILE * ((width + TILE - 1) / TILE), pairs, planes, depth);
+  const float g = row_upstream(upstream, per_token, mean, static_cast<int>(t), live);
+  const float own = target_gradient(rows.miss[row], g);
+  const float a = rounded ? 1.f : g * rows.scale[row];
+  const float b = rounded ? own - bf16_round(own) : own;
+  const int y = target[row];
+  const uint4* wr = reinterpret_cast<const uint4*>(weight + static_cast<int64_t>(y < 0 ? 0 : y) * ld_weight);
   for (int i = lane; i < vecs; i += 32) {
     float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     for (int s = 0; s < parts; ++s) {
@@ -663,21 +730,19 @@ __global__ void __launch_bounds__(256) vocab_finish(const float* __restrict__ ac
       const float4 u = __ldcs(from), w = __ldcs(from + 1);
       v[0] += u.x, v[1] += u.y, v[2] += u.z, v[3] += u.w, v[4] += w.x, v[5] += w.y, v[6] += w.z, v[7] += w.w;
     }
-    if (wr != nullptr) {
-      const uint4 k = wr[i];
-      v[0] = a * v[0] - b * bf16_lo(k.x), v[1] = a * v[1] - b * bf16_hi(k.x);
-      v[2] = a * v[2] - b * bf16_lo(k.y), v[3] = a * v[3] - b * bf16_hi(k.y);
-      v[4] = a * v[4] - b * bf16_lo(k.z), v[5] = a * v[5] - b * bf16_hi(k.z);
-      v[6] = a * v[6] - b * bf16_lo(k.w), v[7] = a * v[7] - b * bf16_hi(k.w);
-    }
+    const uint4 k = wr[i];
+    v[0] = a * v[0] + b * bf16_lo(k.x), v[1] = a * v[1] + b * bf16_hi(k.x);
+    v[2] = a * v[2] + b * bf16_lo(k.y), v[3] = a * v[3] + b * bf16_hi(k.y);
+    v[4] = a * v[4] + b * bf16_lo(k.z), v[5] = a * v[5] + b * bf16_hi(k.z);
+    v[6] = a * v[6] + b * bf16_lo(k.w), v[7] = a * v[7] + b * bf16_hi(k.w);
     to[i] = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
                        pack_bf16x2(v[6], v[7]));
   }
 }
 
 template <int MODE, bool REDO>
-static int launch(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& out, const Params& p, int pairs,
-                  cudaStream_t s) {
+static int launch(const CUtensorMap& a, const CUtensorMap& a32, const CUtensorMap& b, const CUtensorMap& out,
+                  const Params& p, int pairs, cudaStream_t s) {
   auto kern = vocab_product<MODE, REDO>;
   static uint64_t configured = 0;  // per device: a function's attributes are set on the current one
   int device = 0;
@@ -689,7 +754,7 @@ static int launch(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap&
     }
     if (device < 64) configured |= uint64_t(1) << device;
   }
-  kern<<<2 * pairs, THREADS, SMEM_BYTES, s>>>(a, b, out, p);
+  kern<<<2 * pairs, THREADS, SMEM_BYTES, s>>>(a, a32, b, out, p);
   return launch_status();
 }
 
@@ -713,12 +778,8 @@ constexpr int64_t kPlaneBytes = int64_t(1) << 29;
 constexpr int kMostPlanes = 16;
 
 int pairs_of_device(int* pairs) {
-  int device = 0, sms = 0;
-  if (cudaGetDevice(&device) != cudaSuccess ||
-      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) {
-    cudaGetLastError();
-    return MEEP2B_ERR_LAUNCH;
-  }
+  int sms = 0;
+  MEEP2B_TRY(device_sms(&sms));
   *pairs = sms / 2 > 0 ? sms / 2 : 1;
   return MEEP2B_OK;
 }
@@ -747,20 +808,24 @@ vocab::Params params_of(const meep2b_linear_ce* a) {
   p.part = a->part, p.rows_pad = a->rows_pad, p.upstream = a->upstream;
   p.per_token = a->reduction == MEEP2B_REDUCE_NONE, p.mean = a->reduction == MEEP2B_REDUCE_MEAN;
   p.vocab = static_cast<int>(a->vocab), p.hidden = static_cast<int>(a->hidden_size), p.planes = a->planes;
+  p.depth = static_cast<int>(a->piece_cols > 0 && a->piece_cols < a->vocab ? a->piece_cols : a->vocab);
   return p;
 }
 
 struct CeMaps {
-  CUtensorMap rows, rows_mn, head, head_mn, piece, piece_mn, piece_out, acc, d_weight;
+  CUtensorMap rows, rows32, rows_mn, head, head_mn, piece, piece32, piece_mn, piece_out, acc, d_weight;
 };
 
 int maps_of(const meep2b_linear_ce* a, CeMaps* m, bool acc, bool d_weight) {
   using vocab::map_bf16;
   const int64_t H = a->hidden_size;
   MEEP2B_TRY(map_bf16(&m->rows, a->compact, H, a->rows_pad, H, 64, 128, CU_TENSOR_MAP_SWIZZLE_128B));
+  MEEP2B_TRY(map_bf16(&m->rows32, a->compact, H, a->rows_pad, H, 64, 32, CU_TENSOR_MAP_SWIZZLE_128B));
   MEEP2B_TRY(map_bf16(&m->head, a->weight, H, a->vocab, a->ld_weight, 64, 128, CU_TENSOR_MAP_SWIZZLE_128B));
   if (a->piece != nullptr) {
     MEEP2B_TRY(map_bf16(&m->piece, a->piece, a->piece_cols, a->rows_pad, a->piece_cols, 64, 128,
+                        CU_TENSOR_MAP_SWIZZLE_128B));
+    MEEP2B_TRY(map_bf16(&m->piece32, a->piece, a->piece_cols, a->rows_pad, a->piece_cols, 64, 32,
                         CU_TENSOR_MAP_SWIZZLE_128B));
     MEEP2B_TRY(map_bf16(&m->piece_out, a->piece, a->piece_cols, a->rows_pad, a->piece_cols, 32, 32,
                         CU_TENSOR_MAP_SWIZZLE_64B));
@@ -830,24 +895,29 @@ int meep2b_linear_ce_forward(const meep2b_linear_ce* a, void* stream) {
   if (grad && (a->piece == nullptr || a->planes < 1)) return MEEP2B_ERR_SHAPE;
   const vocab::Rows rows = rows_of(a);
   const int row_tiles = static_cast<int>(a->rows_pad / vocab::TILE);
-  vocab::vocab_scan<<<1, 1024, 0, s>>>(a->targets, a->tokens, a->ignore_index, a->source, a->slot, a->state, a->flags,
-                                       row_tiles, per_token ? a->loss : nullptr);
-  MEEP2B_TRY(launch_status());
-  const int slots = 2 * static_cast<int>((a->vocab + vocab::TILE - 1) / vocab::TILE);
-  if (a->tokens > 0) {
-    vocab::vocab_gather<<<static_cast<unsigned>(a->rows_pad / 8), 256, 0, s>>>(
-        static_cast<const __nv_bfloat16*>(a->hidden), a->ld_hidden, static_cast<const __nv_bfloat16*>(a->weight),
-        a->ld_weight, a->targets, static_cast<int>(a->vocab), static_cast<int>(a->hidden_size), a->state, a->source,
-        static_cast<__nv_bfloat16*>(a->compact), a->target, rows);
+  const bool small = a->tokens > 0 && a->tokens <= vocab::kScanned;
+  if (!small) {
+    vocab::vocab_scan<<<1, 1024, 0, s>>>(a->targets, a->tokens, a->ignore_index, a->source, a->slot, a->state, a->flags,
+                                         row_tiles, per_token ? a->loss : nullptr);
     MEEP2B_TRY(launch_status());
-    int pairs = 0;
-    MEEP2B_TRY(pairs_of_device(&pairs));
-    CeMaps m;
+  }
+  const int slots = 2 * static_cast<int>((a->vocab + vocab::TILE - 1) / vocab::TILE);
+  int pairs = 0;
+  MEEP2B_TRY(pairs_of_device(&pairs));
+  CeMaps m;
+  if (a->tokens > 0) {
     MEEP2B_TRY(maps_of(a, &m, grad, false));
+    auto gather = small ? vocab::vocab_gather<true> : vocab::vocab_gather<false>;
+    gather<<<static_cast<unsigned>(a->rows_pad / 8), 256, 0, s>>>(
+        static_cast<const __nv_bfloat16*>(a->hidden), a->ld_hidden, static_cast<const __nv_bfloat16*>(a->weight),
+        a->ld_weight, a->targets, static_cast<int>(a->tokens), a->ignore_index, static_cast<int>(a->vocab),
+        static_cast<int>(a->hidden_size), a->state, a->flags, row_tiles, a->source, a->slot,
+        per_token ? a->loss : nullptr, static_cast<__nv_bfloat16*>(a->compact), a->target, rows);
+    MEEP2B_TRY(launch_status());
     MEEP2B_TRY(each_piece(a, params_of(a), [&](const vocab::Params& p) -> int {
-      if (!grad) return vocab::launch<vocab::kStats, false>(m.rows, m.head, m.piece_out, p, pairs, s);
-      MEEP2B_TRY((vocab::launch<vocab::kProbs, false>(m.rows, m.head, m.piece_out, p, pairs, s)));
-      return vocab::launch<vocab::kAcc, false>(m.piece, m.head_mn, m.acc, p, pairs, s);
+      if (!grad) return vocab::launch<vocab::kStats, false>(m.rows, m.rows32, m.head, m.piece_out, p, pairs, s);
+      MEEP2B_TRY((vocab::launch<vocab::kProbs, false>(m.rows, m.rows32, m.head, m.piece_out, p, pairs, s)));
+      return vocab::launch<vocab::kAcc, false>(m.piece, m.piece32, m.head_mn, m.acc, p, pairs, s);
     }));
   }
   const unsigned join = static_cast<unsigned>(a->tokens > 0 ? (a->tokens + 31) / 32 : 1);
@@ -856,13 +926,9 @@ int meep2b_linear_ce_forward(const meep2b_linear_ce* a, void* stream) {
                                           a->reduction == MEEP2B_REDUCE_MEAN);
   MEEP2B_TRY(launch_status());
   if (grad && a->tokens > 0) {
-    int pairs = 0;
-    MEEP2B_TRY(pairs_of_device(&pairs));
-    CeMaps m;
-    MEEP2B_TRY(maps_of(a, &m, true, false));
     MEEP2B_TRY(each_piece(a, params_of(a), [&](const vocab::Params& p) -> int {
-      MEEP2B_TRY((vocab::launch<vocab::kReprobs, true>(m.rows, m.head, m.piece_out, p, pairs, s)));
-      return vocab::launch<vocab::kAcc, true>(m.piece, m.head_mn, m.acc, p, pairs, s);
+      MEEP2B_TRY((vocab::launch<vocab::kReprobs, true>(m.rows, m.rows32, m.head, m.piece_out, p, pairs, s)));
+      return vocab::launch<vocab::kAcc, true>(m.piece, m.piece32, m.head_mn, m.acc, p, pairs, s);
     }));
   }
   return MEEP2B_OK;
@@ -887,18 +953,18 @@ int meep2b_linear_ce_backward(const meep2b_linear_ce* a, void* stream) {
     CeMaps m;
     MEEP2B_TRY(maps_of(a, &m, a->d_hidden != nullptr, true));
     MEEP2B_TRY(each_piece(a, params_of(a), [&](const vocab::Params& p) -> int {
-      MEEP2B_TRY((vocab::launch<vocab::kGrad, false>(m.rows, m.head, m.piece_out, p, pairs, s)));
+      MEEP2B_TRY((vocab::launch<vocab::kGrad, false>(m.rows, m.rows32, m.head, m.piece_out, p, pairs, s)));
       if (a->d_hidden != nullptr)
-        MEEP2B_TRY((vocab::launch<vocab::kAcc, false>(m.piece, m.head_mn, m.acc, p, pairs, s)));
-      return vocab::launch<vocab::kWeight, false>(m.piece_mn, m.rows_mn, m.d_weight, p, pairs, s);
+        MEEP2B_TRY((vocab::launch<vocab::kAcc, false>(m.piece, m.piece32, m.head_mn, m.acc, p, pairs, s)));
+      return vocab::launch<vocab::kWeight, false>(m.piece_mn, m.piece_mn, m.rows_mn, m.d_weight, p, pairs, s);
     }));
   }
   if (a->d_hidden != nullptr && a->tokens > 0) {
     const vocab::Params p = params_of(a);
     vocab::vocab_finish<<<static_cast<unsigned>((a->tokens + 7) / 8), 256, 0, s>>>(
-        a->acc, pairs, a->planes, a->rows_pad, static_cast<int>(a->hidden_size), a->tokens, a->state, a->slot,
-        a->target, p.rows, recompute ? nullptr : static_cast<const __nv_bfloat16*>(a->weight), a->ld_weight,
-        a->upstream, p.per_token, p.mean, static_cast<__nv_bfloat16*>(a->d_hidden));
+        a->acc, pairs, a->planes, p.depth, a->rows_pad, static_cast<int>(a->hidden_size), a->tokens, a->state, a->slot,
+        a->target, p.rows, static_cast<const __nv_bfloat16*>(a->weight), a->ld_weight, a->upstream, p.per_token, p.mean,
+        recompute, static_cast<__nv_bfloat16*>(a->d_hidden));
     MEEP2B_TRY(launch_status());
   }
   return MEEP2B_OK;

@@ -1,11 +1,13 @@
 """The fine-tuning step's operators without a GPU: the buffers the vocabulary loss plans, and the refusal to run on the
 CPU."""
 
+import ctypes
+
 import pytest
 import torch
 
 import meepsquared_b200 as mb
-from meepsquared_b200 import _loss
+from meepsquared_b200 import _lib, _loss
 
 
 @pytest.mark.parametrize("tokens", [1, 255, 256, 257, 4096, 16384, 1 << 20])
@@ -26,6 +28,21 @@ def test_sizes_beyond_the_entry_point_are_refused():
         _loss._plan(1 << 25, 64, 1000)
     with pytest.raises(ValueError):
         _loss._plan(16, 0, 1000)
+
+
+@pytest.mark.parametrize("cls", [_lib.Balance, _lib.HeadNorm, _lib.LinearCE])
+def test_packed_arguments_are_the_structures_bytes(cls):
+    pack = _lib.packer(cls)
+    values, n = [], 1
+    filled = cls()
+    for name, kind in cls._fields_:
+        count = getattr(kind, "_length_", 1)
+        some = [float(n + i) if kind is ctypes.c_float else n + i for i in range(count)]
+        setattr(filled, name, kind(*some) if count > 1 else some[0])
+        values += some
+        n += count
+    got = pack.pack(*values)
+    assert got == bytes(filled)[:len(got)] and not any(bytes(filled)[len(got):])
 
 
 def test_no_cpu_fallback():
