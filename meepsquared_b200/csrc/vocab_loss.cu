@@ -24,6 +24,10 @@
 //   kGrad     g (q / Z - [v = y]) as bf16 into the piece's buffer (the head's gradient, and dh beside it)
 //   kAcc      dh's product: piece x W, float32, stored by the first piece and added (TMA reduction) by the others
 //   kWeight   dW's product: piece^T x h, bf16
+//
+// The tensor cores cut every step's sum off toward zero. Over the 256 steps of a logit of 4,096 products that made the
+// mean loss 1.1e-6 of itself too small; so beyond 2,048 products a logit's sum is taken from tensor memory every 2,048
+// and joined in the epilogue's registers (DEEP), with ordinary float32 additions.
 #include "common.cuh"
 #include "host.hpp"
 
@@ -44,6 +48,7 @@ constexpr int NUM_BARS = 2 * STAGES + 5;
 constexpr int OFF_TMEM = OFF_BAR + NUM_BARS * 8;
 constexpr int SMEM_BYTES = OFF_TMEM + 16 + 1024;
 constexpr uint32_t TMEM_COLS = 512;
+constexpr int DEEP_BLOCKS = 32;  // k-blocks (2,048 products) that a logit is summed over in tensor memory
 constexpr int GROUP = 8;  // row tiles that share a column tile before the next column tile is taken
 static_assert(SMEM_BYTES <= 232448, "shared memory plan exceeds 227 KB");
 
@@ -54,7 +59,7 @@ constexpr float kWindow = 7.9228162514264338e28f;  // 2^96
 enum Mode { kStats, kProbs, kReprobs, kGrad, kAcc, kWeight };
 
 // ints of `state`
-enum { kLive = 0, kRedo = 1, kDone = 2, kStateInts = 8 };
+enum { kLive = 0, kRedo = 1, kDone = 2, kParts = 3, kStateInts = 8 };  // (kParts: planes that kAcc wrote)
 
 struct Rows {  // per live row, float32
   float* ref;    // the reference of q, in units of log 2 (after a recomputation: the row's log-sum)
@@ -65,7 +70,7 @@ struct Rows {  // per live row, float32
 };
 
 struct Params {
-  const int32_t* state;
+  int32_t* state;
   const int32_t* flags;    // row tiles to compute again
   const int32_t* target;   // per live row (-1 past the last)
   const int32_t* source;   // the live row's token
@@ -137,6 +142,12 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
+// The kernels of a call are launched as programmatic dependents of one another: the next one's CTAs may take their
+// places (and set up barriers and tensor memory) while this one runs out, and wait here, before they touch any memory,
+// until all of this one's work is done and visible.
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_last() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 __device__ __forceinline__ void tma_add_2d(const CUtensorMap* map, uint32_t src, int32_t c0, int32_t c1) {
   asm volatile("cp.reduce.async.bulk.tensor.2d.global.shared::cta.add.tile.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
                    reinterpret_cast<uint64_t>(map)),
@@ -176,10 +187,11 @@ __device__ __forceinline__ float row_upstream(const float* upstream, int per_tok
 __device__ __forceinline__ float target_gradient(float miss, float g) { return __fmul_rn(-miss, g); }
 
 // One unit's epilogue for one warp: 32 rows (a lane each) and 128 columns, 32 at a time.
-template <int MODE>
+// held (DEEP): the unit's sums, already out of tensor memory.
+template <int MODE, bool DEEP>
 __device__ __forceinline__ void epilogue(const Params& p, const CUtensorMap* out, int m, int n, int part, bool empty,
                                          int row0, int half, uint32_t acc, int lane, uint32_t stg, uint32_t tempty,
-                                         int live) {
+                                         int live, float (&held)[4][32]) {
   const int row = row0 + lane;  // of the live rows (kWeight: of the piece's columns)
   constexpr bool LOGITS = MODE == kStats || MODE == kProbs || MODE == kReprobs || MODE == kGrad;
   const int c_first = n * TILE + half * 128;  // column of the product
@@ -194,14 +206,19 @@ __device__ __forceinline__ void epilogue(const Params& p, const CUtensorMap* out
     }
   }
   float sum = 0.f, far = -INFINITY;  // the sum within the window; log2 of what lies above it, against the reference
-#pragma unroll 1
+#pragma unroll(DEEP ? 4 : 1)
   for (int c = 0; c < 4; ++c) {
     const int col = c_first + 32 * c;
     float v[32];
-    tmem_ld32(acc + 32 * c, v);
-    if (c == 3) {
-      tc_fence_before();
-      mbar_arrive_remote(tempty, 0);  // the whole accumulator has been read
+    if (DEEP) {
+#pragma unroll
+      for (int j = 0; j < 32; ++j) v[j] = held[c][j];
+    } else {
+      tmem_ld32(acc + 32 * c, v);
+      if (c == 3) {
+        tc_fence_before();
+        mbar_arrive_remote(tempty, 0);  // the whole accumulator has been read
+      }
     }
     if (LOGITS) {
       const int vcol = p.v0 + col;  // of the vocabulary
@@ -301,13 +318,17 @@ __device__ __forceinline__ void epilogue(const Params& p, const CUtensorMap* out
   }
 }
 
-template <int MODE, bool REDO>
+template <int MODE, bool REDO, bool DEEP>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     vocab_product(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap ta32,
                   const __grid_constant__ CUtensorMap tb, const __grid_constant__ CUtensorMap tout, const Params p) {
   constexpr bool A_MN = MODE == kWeight;
   constexpr bool B_MN = MODE == kWeight || MODE == kAcc;
-  if (REDO && p.state[kRedo] == 0) return;
+  if (REDO) {
+    let_next_start();
+    wait_for_last();
+    if (p.state[kRedo] == 0) return;
+  }
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t sbase = smem_u32(smem);
@@ -343,11 +364,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
   cluster_sync();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  if (!REDO) {
+    let_next_start();
+    wait_for_last();
+  }
   const Units w = units_of<MODE>(p, pairs);
   const int live = p.state[kLive];
+  if (MODE == kAcc && blockIdx.x == 0 && threadIdx.x == 0) p.state[kParts] = w.parts;
 
-  if (warp == 0) {
-    if (lane == 0) {  // ---------------------------------------------------------------------- TMA producer (each CTA)
+  // DEEP: the epilogue's warpgroups take 208 registers a thread, the first one keeps 88: 384 x 168 in all, what the
+  // kernel is launched with (checked there)
+  if (warp < EPI_WARP0) {
+    if (DEEP) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    if (warp == 0 && lane == 0) {  // ---------------------------------------------------------------------- TMA producer (each CTA)
       tma_prefetch_desc(&ta);
       tma_prefetch_desc(&tb);
       int stage = 0;
@@ -397,9 +426,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
       if (!ok && rank == 0)
         for (int s = 0; s < STAGES; ++s)
           if (issued[s]) mbar_wait_drain(bar_full(s), last_parity[s]);
-    }
-  } else if (warp == 1) {
-    if (lane == 0 && rank == 0) {  // -------------------------------------------------------- MMA issuer (the leader)
+    } else if (warp == 1 && lane == 0 && rank == 0) {  // -------------------------------------------------------- MMA issuer (the leader)
       constexpr uint32_t IDESC = idesc_bf16(256, 256, A_MN, B_MN);
       const uint64_t a_desc0 = A_MN ? smem_desc(sbase, 8192, 1024, 2) : smem_desc(sbase, 16, 1024, 2);
       const uint64_t b_desc0 = B_MN ? smem_desc(sbase + OPERAND_BYTES, 8192, 1024, 2)
@@ -413,32 +440,37 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         int m, n, part;
         w.decode(u, m, n, part);
         if (REDO && p.flags[m] == 0) continue;
-        const int ab = it & 1;
-        if (!mbar_wait_cluster(bar_tempty(ab), ((it >> 1) & 1) ^ 1)) { ok = false; break; }
-        tc_fence_after();
-        const uint32_t d = tmem_base + ab * TILE;
-        const int k0 = w.k_begin(part), k1 = w.k_begin(part + 1);
-        for (int kb = k0; kb < k1; ++kb) {
-          if (!mbar_wait(bar_full(stage), phase)) { ok = false; break; }
+        const int passes = DEEP ? (w.kblocks + DEEP_BLOCKS - 1) / DEEP_BLOCKS : 1;
+        for (int pass = 0; pass < passes && ok; ++pass) {
+          const int ab = it & 1;
+          if (!mbar_wait_cluster(bar_tempty(ab), ((it >> 1) & 1) ^ 1)) { ok = false; break; }
           tc_fence_after();
-          const uint64_t a_st = a_desc0 + static_cast<uint32_t>(stage) * (STAGE_BYTES / 16);
-          const uint64_t b_st = b_desc0 + static_cast<uint32_t>(stage) * (STAGE_BYTES / 16);
-          mma_bf16_pair(d, a_st, b_st, IDESC, kb != k0);
+          const uint32_t d = tmem_base + ab * TILE;
+          const int k0 = DEEP ? w.kblocks * pass / passes : w.k_begin(part);
+          const int k1 = DEEP ? w.kblocks * (pass + 1) / passes : w.k_begin(part + 1);
+          for (int kb = k0; kb < k1; ++kb) {
+            if (!mbar_wait(bar_full(stage), phase)) { ok = false; break; }
+            tc_fence_after();
+            const uint64_t a_st = a_desc0 + static_cast<uint32_t>(stage) * (STAGE_BYTES / 16);
+            const uint64_t b_st = b_desc0 + static_cast<uint32_t>(stage) * (STAGE_BYTES / 16);
+            mma_bf16_pair(d, a_st, b_st, IDESC, kb != k0);
 #pragma unroll
-          for (int kk = 1; kk < BK / 16; ++kk) mma_bf16_pair(d, a_st + A_KK * kk, b_st + B_KK * kk, IDESC, 1);
-          mma_commit_pair(bar_empty(stage));
-          if (++stage == STAGES) stage = 0, phase ^= 1;
+            for (int kk = 1; kk < BK / 16; ++kk) mma_bf16_pair(d, a_st + A_KK * kk, b_st + B_KK * kk, IDESC, 1);
+            mma_commit_pair(bar_empty(stage));
+            if (++stage == STAGES) stage = 0, phase ^= 1;
+          }
+          if (!ok) break;
+          mma_commit_pair(bar_tfull(ab));
+          ++it;
         }
-        if (!ok) break;
-        mma_commit_pair(bar_tfull(ab));
-        ++it;
       }
       if (!ok) {
         mma_commit_pair(bar_drain);
         mbar_wait_drain(bar_drain, 0);
       }
     }
-  } else if (warp >= EPI_WARP0) {  // --------------------------------------------------------- epilogue (each CTA)
+  } else {  // ------------------------------------------------------------------------------- epilogue (each CTA)
+    if (DEEP) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     const int q = warp & 3, half = (warp - EPI_WARP0) >> 2;
     const uint32_t stg = sbase + OFF_STG + static_cast<uint32_t>(warp - EPI_WARP0) * STG_BYTES;
     int it = 0;
@@ -446,12 +478,40 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
       int m, n, part;
       w.decode(u, m, n, part);
       if (REDO && p.flags[m] == 0) continue;
+      float held[4][32];
+      if (DEEP) {
+        const int passes = (w.kblocks + DEEP_BLOCKS - 1) / DEEP_BLOCKS;
+        bool ok = true;
+#pragma unroll
+        for (int c = 0; c < 128; ++c) held[c / 32][c % 32] = 0.f;
+        for (int pass = 0; pass < passes; ++pass, ++it) {
+          const int ab = it & 1;
+          ok = mbar_wait(bar_tfull(ab), (it >> 1) & 1);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t acc = tmem_base + ab * TILE + half * 128 + (static_cast<uint32_t>(32 * q) << 16);
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            float v[16];
+            tmem_ld16(acc + 16 * c, v);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) held[c / 2][16 * (c % 2) + j] += v[j];
+          }
+          tc_fence_before();
+          mbar_arrive_remote(bar_tempty(ab), 0);
+        }
+        if (!ok) break;
+        epilogue<MODE, DEEP>(p, &tout, m, n, part, false, m * TILE + 128 * static_cast<int>(rank) + 32 * q, half, 0u,
+                             lane, stg, 0u, live, held);
+        continue;
+      }
       const int ab = it & 1;
       if (!mbar_wait(bar_tfull(ab), (it >> 1) & 1)) break;
       tc_fence_after();
       const uint32_t acc = tmem_base + ab * TILE + half * 128 + (static_cast<uint32_t>(32 * q) << 16);
-      epilogue<MODE>(p, &tout, m, n, part, w.k_begin(part) == w.k_begin(part + 1),
-                     m * TILE + 128 * static_cast<int>(rank) + 32 * q, half, acc, lane, stg, bar_tempty(ab), live);
+      epilogue<MODE, DEEP>(p, &tout, m, n, part, w.k_begin(part) == w.k_begin(part + 1),
+                           m * TILE + 128 * static_cast<int>(rank) + 32 * q, half, acc, lane, stg, bar_tempty(ab), live,
+                           held);
       ++it;
     }
     if (lane == 0) bulk_wait_all();
@@ -500,6 +560,7 @@ __global__ void __launch_bounds__(1024) vocab_scan(const int64_t* __restrict__ t
                                                   int32_t* __restrict__ flags, int row_tiles,
                                                   float* __restrict__ token_loss) {
   __shared__ int words[32];
+  let_next_start();
   const int64_t per = (tokens + 1023) / 1024;
   const int64_t t0 = min(tokens, per * threadIdx.x), t1 = min(tokens, t0 + per);
   int mine = 0;
@@ -535,6 +596,8 @@ __global__ void __launch_bounds__(256) vocab_gather(const __nv_bfloat16* __restr
   const int lane = threadIdx.x & 31;
   const int row = blockIdx.x * 8 + (threadIdx.x >> 5);
   int live, from = 0;
+  let_next_start();
+  wait_for_last();
   if (SCAN) {
     __shared__ int words[8], mine_rows[8];
     const int per = (tokens + 255) / 256;
@@ -615,11 +678,13 @@ __global__ void __launch_bounds__(1024) vocab_join(const float* __restrict__ par
   __shared__ double reduce[32];
   __shared__ bool last;
   const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
+  let_next_start();
+  wait_for_last();
   const int live = state[kLive];
-  const int row = blockIdx.x * 32 + x;
-  if (row < live) {
+  {
+    const int row = blockIdx.x * 32 + x;
     float sum = 0.f, far = -INFINITY;
-    for (int s0 = y; s0 < slots; s0 += 32 * 16) {
+    for (int s0 = y; row < live && s0 < slots; s0 += 32 * 16) {
       float v[16];
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
@@ -636,43 +701,48 @@ __global__ void __launch_bounds__(1024) vocab_join(const float* __restrict__ par
         }
       }
     }
-    sums[y][x] = sum, fars[y][x] = far;
+    sums[x][y] = sum, fars[x][y] = far;
   }
   __syncthreads();
-  if (y == 0 && row < live) {
-    float sum = 0.f, far = -INFINITY;
-    for (int i = 0; i < 32; ++i) {
-      sum += sums[i][x];
-      const float f = fars[i][x];
-      if (f != -INFINITY) {
+  const int row = blockIdx.x * 32 + y;  // from here a warp a row
+  if (row < live) {
+    float sum = sums[y][x], far = fars[y][x];
+    const bool any = __any_sync(0xffffffffu, far != -INFINITY);
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) {
+      sum += __shfl_xor_sync(0xffffffffu, sum, off);
+      if (any) {
+        const float f = __shfl_xor_sync(0xffffffffu, far, off);
         const float hi = fmaxf(far, f), lo = fminf(far, f);
-        far = hi + log2f(1.0f + exp2f(lo - hi));
+        if (hi != -INFINITY) far = hi + log2f(1.0f + exp2f(lo - hi));
       }
     }
-    // the reference was rounded to a multiple of log 2: what the rounding took is put back
-    const float ref = rows.ref[row], logit = rows.logit[row];
-    const float off = fmaf(logit, kLog2e, -ref);
-    float value;
-    if (far == -INFINITY) {
-      sum *= exp2f(-off);
-      const float z = 1.0f + sum;
-      value = log1pf(sum);
-      rows.lse[row] = fmaf(logit, kLog2e, log2f(z));
-      rows.scale[row] = exp2f(-off) / z;
-      rows.miss[row] = sum / z;
-    } else {
-      const float more = far + log2f(1.0f + (1.0f + sum) * exp2f(-far)) - off;
-      value = more * kLn2;
-      const float lse = fmaf(logit, kLog2e, more);
-      rows.lse[row] = lse;
-      rows.ref[row] = lse;
-      rows.scale[row] = 1.0f;
-      rows.miss[row] = 1.0f - exp2f(-more);
-      flags[row / TILE] = 1;
-      state[kRedo] = 1;
+    if (x == 0) {
+      // the reference was rounded to a multiple of log 2: what the rounding took is put back
+      const float ref = rows.ref[row], logit = rows.logit[row];
+      const float off = fmaf(logit, kLog2e, -ref);
+      float value;
+      if (!any) {
+        sum *= exp2f(-off);
+        const float z = 1.0f + sum;
+        value = log1pf(sum);
+        rows.lse[row] = fmaf(logit, kLog2e, log2f(z));
+        rows.scale[row] = exp2f(-off) / z;
+        rows.miss[row] = sum / z;
+      } else {
+        const float more = far + log2f(1.0f + (1.0f + sum) * exp2f(-far)) - off;
+        value = more * kLn2;
+        const float lse = fmaf(logit, kLog2e, more);
+        rows.lse[row] = lse;
+        rows.ref[row] = lse;
+        rows.scale[row] = 1.0f;
+        rows.miss[row] = 1.0f - exp2f(-more);
+        flags[row / TILE] = 1;
+        state[kRedo] = 1;
+      }
+      if (token_loss != nullptr) token_loss[source[row]] = value;
+      else row_loss[row] = value;
     }
-    if (token_loss != nullptr) token_loss[source[row]] = value;
-    else row_loss[row] = value;
   }
   if (token_loss != nullptr) return;
   __threadfence();
@@ -697,65 +767,102 @@ __global__ void __launch_bounds__(1024) vocab_join(const float* __restrict__ par
 
 // dh of every token from its row's planes, zero for ignored tokens. From the forward pass's q: g (scale sum_planes -
 // miss W_y). From the product over g (p - [v = y]) in bf16 (`rounded`): the sum, and what the rounding of the target's
-// value took times W_y, which is the largest rounding of a row by far. A warp per token.
-__global__ void __launch_bounds__(256) vocab_finish(const float* __restrict__ acc, int pairs, int planes, int depth,
-                                                   int64_t rows_pad, int width, int64_t tokens,
+// value took times W_y, which is the largest rounding of a row by far. A warp per 256 columns of a token, so that few
+// tokens fill the GPU too.
+__global__ void __launch_bounds__(256) vocab_finish(const float* __restrict__ acc, int64_t rows_pad, int width, int64_t tokens,
                                                    const int32_t* __restrict__ state, const int32_t* __restrict__ slot,
                                                    const int32_t* __restrict__ target, Rows rows,
                                                    const __nv_bfloat16* __restrict__ weight, int64_t ld_weight,
                                                    const float* __restrict__ upstream, int per_token, int mean,
                                                    bool rounded, __nv_bfloat16* __restrict__ d_hidden) {
+  wait_for_last();
   const int lane = threadIdx.x & 31;
-  const int64_t t = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  if (t >= tokens) return;
+  const int chunks = (width + 255) / 256;
+  const int64_t unit = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  const int64_t t = unit / chunks;
+  const int i = static_cast<int>(unit - t * chunks) * 32 + lane;  // of the row's pieces of 8 columns
+  if (t >= tokens || 8 * i >= width) return;
   uint4* to = reinterpret_cast<uint4*>(d_hidden + t * width);
-  const int vecs = width / 8;
   const int row = slot[t];
   if (row < 0) {
-    for (int i = lane; i < vecs; i += 32) to[i] = make_uint4(0, 0, 0, 0);
+    to[i] = make_uint4(0, 0, 0, 0);
     return;
   }
   const int live = state[kLive];
-  const int parts = depth_parts((live + TILE - 1) / TILE * ((width + TILE - 1) / TILE), pairs, planes, depth);
+  const int parts = state[kParts];
   const float g = row_upstream(upstream, per_token, mean, static_cast<int>(t), live);
   const float own = target_gradient(rows.miss[row], g);
   const float a = rounded ? 1.f : g * rows.scale[row];
   const float b = rounded ? own - bf16_round(own) : own;
   const int y = target[row];
   const uint4* wr = reinterpret_cast<const uint4*>(weight + static_cast<int64_t>(y < 0 ? 0 : y) * ld_weight);
-  for (int i = lane; i < vecs; i += 32) {
-    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < parts; ++s) {
-      const float4* from = reinterpret_cast<const float4*>(acc + (s * rows_pad + row) * width) + 2 * i;
-      const float4 u = __ldcs(from), w = __ldcs(from + 1);
-      v[0] += u.x, v[1] += u.y, v[2] += u.z, v[3] += u.w, v[4] += w.x, v[5] += w.y, v[6] += w.z, v[7] += w.w;
+  const uint4 k = wr[i];
+  float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  for (int s0 = 0; s0 < parts; s0 += 4) {
+    float4 u[4], w[4];
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      u[s] = w[s] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (s0 + s < parts) {
+        const float4* from = reinterpret_cast<const float4*>(acc + ((s0 + s) * rows_pad + row) * width) + 2 * i;
+        u[s] = __ldcs(from), w[s] = __ldcs(from + 1);
+      }
     }
-    const uint4 k = wr[i];
-    v[0] = a * v[0] + b * bf16_lo(k.x), v[1] = a * v[1] + b * bf16_hi(k.x);
-    v[2] = a * v[2] + b * bf16_lo(k.y), v[3] = a * v[3] + b * bf16_hi(k.y);
-    v[4] = a * v[4] + b * bf16_lo(k.z), v[5] = a * v[5] + b * bf16_hi(k.z);
-    v[6] = a * v[6] + b * bf16_lo(k.w), v[7] = a * v[7] + b * bf16_hi(k.w);
-    to[i] = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
-                       pack_bf16x2(v[6], v[7]));
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      v[0] += u[s].x, v[1] += u[s].y, v[2] += u[s].z, v[3] += u[s].w;
+      v[4] += w[s].x, v[5] += w[s].y, v[6] += w[s].z, v[7] += w[s].w;
+    }
   }
+  v[0] = a * v[0] + b * bf16_lo(k.x), v[1] = a * v[1] + b * bf16_hi(k.x);
+  v[2] = a * v[2] + b * bf16_lo(k.y), v[3] = a * v[3] + b * bf16_hi(k.y);
+  v[4] = a * v[4] + b * bf16_lo(k.z), v[5] = a * v[5] + b * bf16_hi(k.z);
+  v[6] = a * v[6] + b * bf16_lo(k.w), v[7] = a * v[7] + b * bf16_hi(k.w);
+  to[i] = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
+                     pack_bf16x2(v[6], v[7]));
 }
 
-template <int MODE, bool REDO>
-static int launch(const CUtensorMap& a, const CUtensorMap& a32, const CUtensorMap& b, const CUtensorMap& out,
-                  const Params& p, int pairs, cudaStream_t s) {
-  auto kern = vocab_product<MODE, REDO>;
+// `after`: as a programmatic dependent of the launch before it on the stream (one of this call's, which all wait).
+template <typename... P>
+static int launch_chained(bool after, void (*kern)(P...), unsigned grid, unsigned threads, size_t smem, cudaStream_t s,
+                          P... args) {
+  cudaLaunchAttribute attr = {};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(grid), config.blockDim = dim3(threads), config.dynamicSmemBytes = smem, config.stream = s;
+  config.attrs = &attr, config.numAttrs = after ? 1 : 0;
+  if (cudaLaunchKernelEx(&config, kern, args...) != cudaSuccess) return cudaGetLastError(), MEEP2B_ERR_LAUNCH;
+  return MEEP2B_OK;
+}
+
+template <int MODE, bool REDO, bool DEEP>
+static int launch_product(const CUtensorMap& a, const CUtensorMap& a32, const CUtensorMap& b, const CUtensorMap& out,
+                          const Params& p, int pairs, cudaStream_t s, bool after) {
+  auto kern = vocab_product<MODE, REDO, DEEP>;
   static uint64_t configured = 0;  // per device: a function's attributes are set on the current one
   int device = 0;
   if (cudaGetDevice(&device) != cudaSuccess) return cudaGetLastError(), MEEP2B_ERR_LAUNCH;
   if (device >= 64 || !((configured >> device) & 1)) {
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES) != cudaSuccess) {
+    // DEEP's register split adds up to 168 a thread at launch: with fewer the increase would never be granted
+    cudaFuncAttributes attr;
+    if (cudaFuncGetAttributes(&attr, kern) != cudaSuccess || (DEEP && attr.numRegs != 168) ||
+        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES) != cudaSuccess) {
       cudaGetLastError();
       return MEEP2B_ERR_LAUNCH;
     }
     if (device < 64) configured |= uint64_t(1) << device;
   }
-  kern<<<2 * pairs, THREADS, SMEM_BYTES, s>>>(a, a32, b, out, p);
-  return launch_status();
+  return launch_chained(after, kern, 2u * pairs, THREADS, SMEM_BYTES, s, a, a32, b, out, p);
+}
+
+template <int MODE, bool REDO>
+static int launch(const CUtensorMap& a, const CUtensorMap& a32, const CUtensorMap& b, const CUtensorMap& out,
+                  const Params& p, int pairs, cudaStream_t s, bool after = true) {
+  if constexpr (MODE != kAcc && MODE != kWeight) {
+    if (p.hidden > DEEP_BLOCKS * BK) return launch_product<MODE, REDO, true>(a, a32, b, out, p, pairs, s, after);
+  }
+  return launch_product<MODE, REDO, false>(a, a32, b, out, p, pairs, s, after);
 }
 
 static int map_bf16(CUtensorMap* map, const void* base, int64_t inner, int64_t rows, int64_t ld, uint32_t box_inner,
@@ -896,24 +1003,23 @@ int meep2b_linear_ce_forward(const meep2b_linear_ce* a, void* stream) {
   const vocab::Rows rows = rows_of(a);
   const int row_tiles = static_cast<int>(a->rows_pad / vocab::TILE);
   const bool small = a->tokens > 0 && a->tokens <= vocab::kScanned;
-  if (!small) {
-    vocab::vocab_scan<<<1, 1024, 0, s>>>(a->targets, a->tokens, a->ignore_index, a->source, a->slot, a->state, a->flags,
-                                         row_tiles, per_token ? a->loss : nullptr);
-    MEEP2B_TRY(launch_status());
-  }
+  if (!small)
+    MEEP2B_TRY(vocab::launch_chained(false, vocab::vocab_scan, 1, 1024, 0, s, a->targets, a->tokens, a->ignore_index,
+                                     a->source, a->slot, a->state, a->flags, row_tiles,
+                                     per_token ? a->loss : static_cast<float*>(nullptr)));
   const int slots = 2 * static_cast<int>((a->vocab + vocab::TILE - 1) / vocab::TILE);
   int pairs = 0;
   MEEP2B_TRY(pairs_of_device(&pairs));
   CeMaps m;
   if (a->tokens > 0) {
     MEEP2B_TRY(maps_of(a, &m, grad, false));
-    auto gather = small ? vocab::vocab_gather<true> : vocab::vocab_gather<false>;
-    gather<<<static_cast<unsigned>(a->rows_pad / 8), 256, 0, s>>>(
-        static_cast<const __nv_bfloat16*>(a->hidden), a->ld_hidden, static_cast<const __nv_bfloat16*>(a->weight),
-        a->ld_weight, a->targets, static_cast<int>(a->tokens), a->ignore_index, static_cast<int>(a->vocab),
-        static_cast<int>(a->hidden_size), a->state, a->flags, row_tiles, a->source, a->slot,
-        per_token ? a->loss : nullptr, static_cast<__nv_bfloat16*>(a->compact), a->target, rows);
-    MEEP2B_TRY(launch_status());
+    MEEP2B_TRY(vocab::launch_chained(
+        !small, small ? vocab::vocab_gather<true> : vocab::vocab_gather<false>, static_cast<unsigned>(a->rows_pad / 8),
+        256, 0, s, static_cast<const __nv_bfloat16*>(a->hidden), a->ld_hidden,
+        static_cast<const __nv_bfloat16*>(a->weight), a->ld_weight, a->targets, static_cast<int>(a->tokens),
+        a->ignore_index, static_cast<int>(a->vocab), static_cast<int>(a->hidden_size), a->state, a->flags, row_tiles,
+        a->source, a->slot, per_token ? a->loss : static_cast<float*>(nullptr),
+        static_cast<__nv_bfloat16*>(a->compact), a->target, rows));
     MEEP2B_TRY(each_piece(a, params_of(a), [&](const vocab::Params& p) -> int {
       if (!grad) return vocab::launch<vocab::kStats, false>(m.rows, m.rows32, m.head, m.piece_out, p, pairs, s);
       MEEP2B_TRY((vocab::launch<vocab::kProbs, false>(m.rows, m.rows32, m.head, m.piece_out, p, pairs, s)));
@@ -921,10 +1027,10 @@ int meep2b_linear_ce_forward(const meep2b_linear_ce* a, void* stream) {
     }));
   }
   const unsigned join = static_cast<unsigned>(a->tokens > 0 ? (a->tokens + 31) / 32 : 1);
-  vocab::vocab_join<<<join, 1024, 0, s>>>(a->part, slots, a->rows_pad, a->state, a->flags, a->source, rows,
-                                          per_token ? a->loss : nullptr, a->row_loss, a->loss,
-                                          a->reduction == MEEP2B_REDUCE_MEAN);
-  MEEP2B_TRY(launch_status());
+  MEEP2B_TRY(vocab::launch_chained(
+      true, vocab::vocab_join, join, 1024, 0, s, static_cast<const float*>(a->part), slots, a->rows_pad, a->state,
+      a->flags, static_cast<const int32_t*>(a->source), rows, per_token ? a->loss : static_cast<float*>(nullptr),
+      a->row_loss, a->loss, static_cast<int>(a->reduction == MEEP2B_REDUCE_MEAN)));
   if (grad && a->tokens > 0) {
     MEEP2B_TRY(each_piece(a, params_of(a), [&](const vocab::Params& p) -> int {
       MEEP2B_TRY((vocab::launch<vocab::kReprobs, true>(m.rows, m.rows32, m.head, m.piece_out, p, pairs, s)));
@@ -949,11 +1055,13 @@ int meep2b_linear_ce_backward(const meep2b_linear_ce* a, void* stream) {
     const cudaError_t e = cudaMemsetAsync(a->d_weight, 0, static_cast<size_t>(a->vocab) * a->hidden_size * 2, s);
     return e == cudaSuccess ? MEEP2B_OK : (cudaGetLastError(), MEEP2B_ERR_LAUNCH);
   }
+  bool after = false;
   if (recompute) {
     CeMaps m;
     MEEP2B_TRY(maps_of(a, &m, a->d_hidden != nullptr, true));
     MEEP2B_TRY(each_piece(a, params_of(a), [&](const vocab::Params& p) -> int {
-      MEEP2B_TRY((vocab::launch<vocab::kGrad, false>(m.rows, m.rows32, m.head, m.piece_out, p, pairs, s)));
+      MEEP2B_TRY((vocab::launch<vocab::kGrad, false>(m.rows, m.rows32, m.head, m.piece_out, p, pairs, s, after)));
+      after = true;
       if (a->d_hidden != nullptr)
         MEEP2B_TRY((vocab::launch<vocab::kAcc, false>(m.piece, m.piece32, m.head_mn, m.acc, p, pairs, s)));
       return vocab::launch<vocab::kWeight, false>(m.piece_mn, m.piece_mn, m.rows_mn, m.d_weight, p, pairs, s);
@@ -961,11 +1069,13 @@ int meep2b_linear_ce_backward(const meep2b_linear_ce* a, void* stream) {
   }
   if (a->d_hidden != nullptr && a->tokens > 0) {
     const vocab::Params p = params_of(a);
-    vocab::vocab_finish<<<static_cast<unsigned>((a->tokens + 7) / 8), 256, 0, s>>>(
-        a->acc, pairs, a->planes, p.depth, a->rows_pad, static_cast<int>(a->hidden_size), a->tokens, a->state, a->slot,
-        a->target, p.rows, static_cast<const __nv_bfloat16*>(a->weight), a->ld_weight, a->upstream, p.per_token, p.mean,
-        recompute, static_cast<__nv_bfloat16*>(a->d_hidden));
-    MEEP2B_TRY(launch_status());
+    const int64_t warps = a->tokens * ((a->hidden_size + 255) / 256);
+    MEEP2B_TRY(vocab::launch_chained(
+        after, vocab::vocab_finish, static_cast<unsigned>((warps + 7) / 8), 256, 0, s, static_cast<const float*>(a->acc),
+        a->rows_pad, static_cast<int>(a->hidden_size), a->tokens, static_cast<const int32_t*>(a->state),
+        static_cast<const int32_t*>(a->slot), static_cast<const int32_t*>(a->target), p.rows,
+        static_cast<const __nv_bfloat16*>(a->weight), a->ld_weight, a->upstream, p.per_token, p.mean, recompute,
+        static_cast<__nv_bfloat16*>(a->d_hidden)));
   }
   return MEEP2B_OK;
 }

@@ -95,7 +95,9 @@ def check(h, w, t, reduction, head, seed=3):
 
 @pytest.mark.parametrize("head", [False, True], ids=["frozen", "trained"])
 @pytest.mark.parametrize("tokens,hidden,vocab", [(1, 8, 1), (1, 64, 7), (2, 72, 256), (37, 200, 257), (255, 64, 1000),
-                                                 (257, 128, 513), (300, 512, 5003), (700, 264, 2048)])
+                                                 (257, 128, 513), (300, 512, 5003), (700, 264, 2048),
+                                                 (70, 2048, 300), (70, 2056, 300), (300, 4104, 1000),
+                                                 (5, 8200, 700)])
 def test_losses_and_gradients(tokens, hidden, vocab, head):
     h, w, t = inputs(tokens, hidden, vocab)
     check(h, w, t, "none", head)
@@ -139,14 +141,15 @@ def test_pieces_and_planes(monkeypatch, piece_cols, planes, head):
     check(h, w, t, "none", head)
 
 
+@pytest.mark.parametrize("hidden", [64, 2104])
 @pytest.mark.parametrize("pieces", [False, True], ids=["whole", "pieces"])
-def test_targets_far_below_the_largest_logit(monkeypatch, pieces):
+def test_targets_far_below_the_largest_logit(monkeypatch, pieces, hidden):
     """Logits hundreds above the target's: beyond the window of the target's own reference, in some rows of some
     tiles (the others keep theirs), and far below it."""
     if pieces:
         plan = _loss._plan
         monkeypatch.setattr(_loss, "_plan", lambda *a: (plan(*a)[0], 512, 2))
-    h, w, t = inputs(700, 64, 1500)
+    h, w, t = inputs(700, hidden, 1500)
     far = torch.arange(700, device=DEV) % 97 == 5
     h[far] *= 200.0   # logits of +-600 or so
     h[600:] *= 30.0   # around the window's edge
