@@ -28,7 +28,7 @@ def _vector(w, dtype):
 
 def _new(t):
     """A contiguous tensor of t's shape and type."""
-    return torch.empty_like(t, memory_format=torch.contiguous_format)
+    return t.new_empty(t.shape)
 
 
 def _call(what, q, k, wq, wk, cos, sin, positions, eps, q_out, k_out, back=(0, 0, *_NO_STRIDES, *_NO_STRIDES, 0, 0, 0)):

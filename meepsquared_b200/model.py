@@ -10,7 +10,12 @@ lora_B zero), so that a model without PEFT installed gets the same trainable par
 * ``install(model, rank, alpha)`` adds ``lora_<stack>_lhs`` (experts, out, rank) and ``lora_<stack>_rhs``
   (experts, rank, in) to every experts module (Transformers' ``gate_up_proj (E, 2I, H)`` / ``down_proj (E, H, I)``
   layout, or the transposed one) and makes its forward ``_moe.routed_forward`` with them;
-* ``lora_parameters(model)`` lists them, in the order a data-parallel gradient bucket wants them (each layer's
+* ``install_attention(model)`` makes the attention modules that norm their query and key heads (q_norm, k_norm) do so
+  with the rotation in one pass (``qk_norm_rope``);
+* ``training_loss(model, input_ids, labels)`` is a fine-tuning step's loss without the logits (``linear_cross_entropy``
+  on the last hidden states and the head), with the routers' balance loss and the tokens of every expert
+  (``balance_loss``);
+* ``lora_parameters(model)`` lists the factors, in the order a data-parallel gradient bucket wants them (each layer's
   down-projection factors before its gate/up ones, ``ddp.LoraGradBucket`` segments).
 
 Experts modules of Transformers versions that predate the ``has_gate`` / ``has_bias`` / ``is_transposed``
@@ -25,6 +30,9 @@ import types
 import torch
 
 from . import _moe
+from ._balance import balance_loss
+from ._heads import qk_norm_rope
+from ._loss import linear_cross_entropy
 
 # What makes a module an experts module. The reference asks for ("num_experts", "has_gate", "has_bias",
 # "is_transposed") (_moe.py:31), the attributes of Transformers >= 5.17; an experts module of an older Transformers
@@ -103,3 +111,91 @@ def lora_parameters(model):
             if s in getattr(experts, "lora_stacks", ()):
                 params += [getattr(experts, f"lora_{s}_lhs"), getattr(experts, f"lora_{s}_rhs")]
     return params
+
+
+def attention_modules(model):
+    """(name, module) of every attention module that norms its query and key heads."""
+    parts = ("q_proj", "k_proj", "v_proj", "o_proj", "q_norm", "k_norm", "head_dim")
+    for name, module in model.named_modules():
+        if all(hasattr(module, p) for p in parts):
+            yield name, module
+
+
+def _attention_forward(self, hidden_states, position_embeddings, attention_mask=None, past_key_values=None, **kwargs):
+    """The attention's forward with norms and rotation in one pass between the projections and torch's attention."""
+    batch, length = hidden_states.shape[:2]
+    heads = (batch, length, -1, self.head_dim)
+    q, k, v = (f(hidden_states).view(heads) for f in (self.q_proj, self.k_proj, self.v_proj))
+    cos, sin = position_embeddings  # (1 or batch, length, rotated): both halves alike
+    half = cos.shape[-1] // 2
+    positions = None
+    if cos.shape[0] > 1:
+        positions = torch.arange(batch * length, device=q.device).view(batch, length)
+    cos, sin = (x.reshape(-1, 2 * half)[:, :half] for x in (cos, sin))
+    q, k = qk_norm_rope(q, k, self.q_norm.weight, self.k_norm.weight, cos, sin, positions=positions,
+                        eps=self.q_norm.variance_epsilon)
+    q, k, v = q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2)
+    if past_key_values is not None:
+        k, v = past_key_values.update(k, v, self.layer_idx)
+    if attention_mask is None and 1 < length < k.shape[2]:
+        raise NotImplementedError("several new tokens behind cached ones need an attention mask")
+    out = torch.nn.functional.scaled_dot_product_attention(
+        q, k, v, attn_mask=attention_mask, dropout_p=self.attention_dropout if self.training else 0.0,
+        is_causal=attention_mask is None and length > 1, scale=self.scaling, enable_gqa=True)
+    return self.o_proj(out.transpose(1, 2).reshape(batch, length, -1)), None
+
+
+def install_attention(model) -> int:
+    """qk_norm_rope in every attention module with normed heads (Transformers' Qwen3 layout: rotary pairs (i, i + n),
+    torch's scaled_dot_product_attention behind it); returns how many were patched."""
+    patched = 0
+    for name, module in attention_modules(model):
+        if getattr(module, "sliding_window", None) is not None:
+            raise NotImplementedError(f"{name}: attention within a sliding window")
+        if module.q_norm.variance_epsilon != module.k_norm.variance_epsilon:
+            raise NotImplementedError(f"{name}: norms of different epsilon")
+        module.forward = types.MethodType(_attention_forward, module)
+        patched += 1
+    return patched
+
+
+def _routers(model):
+    """The routers beside the experts modules, in the layers' order."""
+    return [getattr(model.get_submodule(name.rpartition(".")[0]), "gate") for name, _ in experts_modules(model)]
+
+
+def training_loss(model, input_ids, labels, attention_mask=None, balance: float = 0.0, ignore_index: int = -100):
+    """A fine-tuning step's loss of a Transformers causal language model, and the tokens of every expert: (loss, counts).
+
+    The mean cross entropy of predicting labels (B, T) from the hidden states before each (labels are shifted here, as
+    Transformers does; `ignore_index` where there is none), from the head's weight without the logits; plus `balance`
+    times the routers' balance loss over the tokens that attention_mask (B, T) keeps, on the routers' own choices.
+    counts: (layers, experts) int64, or None without balance (nothing is collected then)."""
+    base = model.get_decoder() if hasattr(model, "get_decoder") else model.model
+    head = model.get_output_embeddings()
+    if getattr(head, "bias", None) is not None:
+        raise NotImplementedError("a head with a bias")
+    seen, hooks = [], []
+
+    def collect(router, args, out):
+        # the router gives its probabilities and its choice; its logits are one small product more
+        x = args[0]
+        seen.append((torch.nn.functional.linear(x.reshape(-1, x.shape[-1]), router.weight), out[2]))
+
+    if balance:
+        if getattr(model, "is_gradient_checkpointing", False):
+            raise NotImplementedError("the balance loss with gradient checkpointing: its routers run twice")
+        hooks = [r.register_forward_hook(collect) for r in _routers(model)]
+    try:
+        hidden = base(input_ids=input_ids, attention_mask=attention_mask, use_cache=False).last_hidden_state
+    finally:
+        for h in hooks:
+            h.remove()
+    targets = torch.nn.functional.pad(labels[:, 1:], (0, 1), value=ignore_index)
+    loss = linear_cross_entropy(hidden, head.weight, targets, ignore_index=ignore_index)
+    if not balance:
+        return loss, None
+    logits, index = zip(*seen)
+    mask = None if attention_mask is None else attention_mask.reshape(-1)
+    extra, counts = balance_loss(logits, index[0].shape[1], mask=mask, top_k_index=index)
+    return loss + balance * extra, counts.view(len(logits), -1)

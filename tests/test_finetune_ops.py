@@ -54,3 +54,18 @@ def test_no_cpu_fallback():
     q = torch.zeros((1, 4, 2, 64))
     with pytest.raises(RuntimeError, match="CUDA"):
         mb.qk_norm_rope(q, q, torch.ones(64), torch.ones(64), torch.ones(4, 32), torch.ones(4, 32))
+
+
+def test_attention_modules_are_found_and_patched():
+    from test_model import tiny_qwen3_moe
+
+    model = tiny_qwen3_moe()
+    found = [a for _, a in mb.model.attention_modules(model)]
+    assert len(found) == 2
+    before = [a.forward for a in found]
+    assert mb.model.install_attention(model) == 2
+    assert all(a.forward != b for a, b in zip(found, before))
+    assert len(mb.model._routers(model)) == 2 and all(hasattr(r, "weight") for r in mb.model._routers(model))
+    found[0].sliding_window = 128
+    with pytest.raises(NotImplementedError, match="sliding window"):
+        mb.model.install_attention(model)
