@@ -1,83 +1,12 @@
 """The load-balancing loss of the routers (Transformers' ``load_balancing_loss_func``) and the tokens each expert got,
 over one layer or all of them in one call, with the gradient of the router logits."""
 
-import array
-
 import torch
 
 from . import _lib
 
-_DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
-_pack = _lib.packer(_lib.Balance).pack
+_DTYPES = (torch.float32, torch.bfloat16)
 MAX_LAYERS, MAX_EXPERTS, MAX_TOKENS = 128, 1024, 1 << 27
-
-
-def _table(pointers):
-    """A host array of device pointers; it has to outlive the call that its address goes to."""
-    return array.array("Q", pointers)
-
-
-def _rows(logits):
-    """The layers' logits as contiguous tensors, and the table of their pointers."""
-    rows = [x if x.is_contiguous() else x.contiguous() for x in logits]
-    return rows, _table([x.data_ptr() for x in rows])
-
-
-def _call(what, first, table, top_k, mask, coef, index=0, counts=0, loss=0, workspace=0, upstream=0, grads=0):
-    tokens, experts = first.shape
-    args = _pack(table.buffer_info()[0], len(table), experts, tokens, top_k, _DTYPES[first.dtype],
-                 0 if mask is None else mask.data_ptr(), index, counts, loss, coef, workspace, upstream, grads)
-    _lib.check(getattr(_lib.load(), what)(args, _lib.stream_of(first)), what)
-
-
-def _forward(logits, top_k, mask, index):
-    rows, table = _rows(logits)
-    first = rows[0]
-    dev = first.device
-    experts = first.shape[1]
-    counts = torch.empty((len(rows), experts) if len(rows) > 1 else (experts,), dtype=torch.int64, device=dev)
-    loss = torch.empty((), dtype=torch.float32, device=dev)
-    # the kernel's sums (64-bit), then the coefficients that the backward pass reads
-    work = torch.empty(2 * (experts + 3) + experts, dtype=torch.float32, device=dev)
-    at = work.data_ptr()
-    ids = None if index is None else _table([i.data_ptr() for i in index])
-    _call("meep2b_balance_loss", first, table, top_k, mask, at + 8 * (experts + 3),
-          0 if ids is None else ids.buffer_info()[0], counts.data_ptr(), loss.data_ptr(), at)
-    return loss, counts, work
-
-
-def _backward(ctx, grad, _):
-    work, mask, *logits = ctx.saved_tensors
-    rows, table = _rows(logits)
-    first = rows[0]
-    layers = len(rows)
-    upstream = grad if grad.dtype == torch.float32 else grad.to(torch.float32)
-    if layers == 1:
-        grads = (torch.empty_like(first),)
-        base = grads[0].data_ptr()
-    else:  # one allocation for all layers: the gradients are its slices
-        every = torch.empty((layers, *first.shape), dtype=first.dtype, device=first.device)
-        grads, base = every.unbind(0), every.data_ptr()
-    step = first.numel() * first.element_size()
-    outs = _table(range(base, base + layers * step, step) if step else [base] * layers)
-    _call("meep2b_balance_loss_backward", first, table, ctx.top_k, mask, work.data_ptr() + 8 * (first.shape[1] + 3),
-          upstream=upstream.data_ptr(), grads=outs.buffer_info()[0])
-    need = ctx.needs_input_grad
-    return (None, None, None, *(grads if all(need[3:]) else [g if n else None for g, n in zip(grads, need[3:])]))
-
-
-class _BalanceLoss(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, top_k, mask, index, *logits):
-        loss, counts, work = _forward(logits, top_k, mask, index)
-        ctx.save_for_backward(work, mask, *logits)
-        ctx.top_k = top_k
-        ctx.mark_non_differentiable(counts)
-        return loss, counts
-
-    @staticmethod
-    def backward(ctx, grad, _):
-        return _lib.once(_backward)(ctx, grad, _)
 
 
 def balance_loss(router_logits, top_k: int, mask=None, top_k_index=None):
@@ -111,7 +40,7 @@ def balance_loss(router_logits, top_k: int, mask=None, top_k_index=None):
         if mask.shape != (tokens,) or mask.device != dev:
             raise ValueError(f"mask {tuple(mask.shape)}: ({tokens},) on the logits' device expected")
         mask = (mask if mask.dtype == torch.bool else mask != 0).contiguous()
-    index = None
+    index = []
     if top_k_index is not None:
         index = [top_k_index] if isinstance(top_k_index, torch.Tensor) else list(top_k_index)
         if len(index) != len(logits) or any(i.shape != (tokens, top_k) or i.device != dev for i in index):
@@ -119,6 +48,4 @@ def balance_loss(router_logits, top_k: int, mask=None, top_k_index=None):
         if any(i.is_floating_point() for i in index):
             raise TypeError("top_k_index: integers expected")
         index = [i.to(torch.int64).contiguous() for i in index]
-    if torch.is_grad_enabled() and any(x.requires_grad for x in logits):
-        return _BalanceLoss.apply(top_k, mask, index, *logits)
-    return _forward(logits, top_k, mask, index)[:2]
+    return _lib.native().balance_loss(logits, top_k, mask, index)

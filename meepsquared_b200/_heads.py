@@ -6,76 +6,7 @@ import torch
 
 from . import _lib
 
-_DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
-_pack = _lib.packer(_lib.HeadNorm).pack
-_NO_STRIDES = (0, 0, 0)
-
-
-def _heads(t):
-    """(B, T, heads, dim) that 16-byte loads can address: itself, or a copy."""
-    vec = 16 // t.element_size()
-    b, s, h, d = t.stride()
-    if d == 1 and not (b % vec or s % vec or h % vec) and t.data_ptr() % 16 == 0:
-        return t
-    return t.clone(memory_format=torch.contiguous_format)
-
-
-def _vector(w, dtype):
-    if w.dtype != dtype or not w.is_contiguous():
-        w = w.detach().to(dtype).contiguous()
-    return w if w.data_ptr() % 16 == 0 else w.clone()
-
-
-def _new(t):
-    """A contiguous tensor of t's shape and type."""
-    return t.new_empty(t.shape)
-
-
-def _call(what, q, k, wq, wk, cos, sin, positions, eps, q_out, k_out, back=(0, 0, *_NO_STRIDES, *_NO_STRIDES, 0, 0, 0)):
-    b, t, hq, d = q.shape
-    args = _pack(q.data_ptr(), k.data_ptr(), b, t, hq, k.shape[2], d, cos.shape[1], *q.stride()[:3], *k.stride()[:3],
-                 _DTYPES[q.dtype], _DTYPES[cos.dtype], wq.data_ptr(), wk.data_ptr(), cos.data_ptr(), sin.data_ptr(),
-                 cos.stride(0), sin.stride(0), cos.shape[0], 0 if positions is None else positions.data_ptr(), eps,
-                 q_out.data_ptr(), k_out.data_ptr(), *back)
-    _lib.check(getattr(_lib.load(), what)(args, _lib.stream_of(q)), what)
-
-
-def _forward(q, k, q_weight, k_weight, cos, sin, positions, eps):
-    q, k = _heads(q), _heads(k)
-    q_out, k_out = _new(q), _new(k)
-    _call("meep2b_head_norm_rotate", q, k, _vector(q_weight, q.dtype), _vector(k_weight, q.dtype), cos, sin, positions,
-          eps, q_out, k_out)
-    return q_out, k_out
-
-
-def _backward(ctx, dq_out, dk_out):
-    q, k, q_weight, k_weight, cos, sin, positions = ctx.saved_tensors
-    need = ctx.needs_input_grad
-    q, k, dq_out, dk_out = _heads(q), _heads(k), _heads(dq_out), _heads(dk_out)
-    wq, wk = _vector(q_weight, q.dtype), _vector(k_weight, q.dtype)
-    dq, dk = _new(q), _new(k)
-    dwq = dwk = partial = None
-    sums = (0, 0, 0)
-    if need[2] or need[3]:
-        dwq, dwk = _new(wq), _new(wk)
-        partial = torch.empty(_lib.load().meep2b_head_norm_partials() * q.shape[3], dtype=torch.float32, device=q.device)
-        sums = (dwq.data_ptr(), dwk.data_ptr(), partial.data_ptr())
-    _call("meep2b_head_norm_rotate_backward", q, k, wq, wk, cos, sin, positions, ctx.eps, dq, dk,
-          (dq_out.data_ptr(), dk_out.data_ptr(), *dq_out.stride()[:3], *dk_out.stride()[:3], *sums))
-    return (dq if need[0] else None, dk if need[1] else None, dwq.to(q_weight.dtype) if need[2] else None,
-            dwk.to(k_weight.dtype) if need[3] else None, None, None, None, None)
-
-
-class _QKNormRope(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, q_weight, k_weight, cos, sin, positions, eps):
-        ctx.save_for_backward(q, k, q_weight, k_weight, cos, sin, positions)
-        ctx.eps = eps
-        return _forward(q, k, q_weight, k_weight, cos, sin, positions, eps)
-
-    @staticmethod
-    def backward(ctx, dq_out, dk_out):
-        return _lib.once(_backward)(ctx, dq_out, dk_out)
+_DTYPES = (torch.float32, torch.bfloat16)
 
 
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor, cos: torch.Tensor,
@@ -119,7 +50,4 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_wei
         if positions.dtype not in (torch.int64, torch.int32):
             raise TypeError(f"positions in {positions.dtype}: int64 or int32 expected")
         positions = positions.to(torch.int64).contiguous()
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or q_weight.requires_grad
-                                    or k_weight.requires_grad):
-        return _QKNormRope.apply(q, k, q_weight, k_weight, cos.detach(), sin.detach(), positions, eps)
-    return _forward(q.detach(), k.detach(), q_weight, k_weight, cos, sin, positions, eps)
+    return _lib.native().qk_norm_rope(q, k, q_weight, k_weight, cos.detach(), sin.detach(), positions, eps)

@@ -6,7 +6,6 @@ falls back to another implementation: a missing library or a non-zero status rai
 
 import ctypes
 import os
-import struct
 
 import torch
 
@@ -85,14 +84,6 @@ class HeadNorm(ctypes.Structure):
     ]
 
 
-def packer(cls):
-    """struct.Struct of a ctypes.Structure's fields in order, with the C compiler's padding: its pack(*values) gives the
-    argument's bytes in a tenth of the time that filling the Structure takes (arrays as that many values, NULL as 0)."""
-    codes = {_p: "P", _i64: "q", _i32: "i", _f32: "f"}
-    return struct.Struct("@" + "".join(codes[t] if t in codes else f"{t._length_}{codes[t._type_]}"
-                                       for _, t in cls._fields_))
-
-
 _SIGNATURES = {
     "meep2b_version": (ctypes.c_char_p, []),
     "meep2b_status_string": (ctypes.c_char_p, [ctypes.c_int]),
@@ -129,17 +120,16 @@ _SIGNATURES = {
     "meep2b_grouped_product_f8": (ctypes.c_int, [ctypes.POINTER(ProductF8), _p]),
     "meep2b_swiglu": (ctypes.c_int, [_p, _i64, _i64, _p, _p]),
     "meep2b_swiglu_backward": (ctypes.c_int, [_p, _p, _i64, _i64, _p, _p]),
-    # (the arguments of the next six are packed: packer(Balance), packer(HeadNorm), packer(LinearCE))
     "meep2b_balance_workspace_bytes": (_sz, [_i32]),
-    "meep2b_balance_loss": (ctypes.c_int, [_p, _p]),
-    "meep2b_balance_loss_backward": (ctypes.c_int, [_p, _p]),
+    "meep2b_balance_loss": (ctypes.c_int, [ctypes.POINTER(Balance), _p]),
+    "meep2b_balance_loss_backward": (ctypes.c_int, [ctypes.POINTER(Balance), _p]),
     "meep2b_head_norm_partials": (ctypes.c_int, []),
-    "meep2b_head_norm_rotate": (ctypes.c_int, [_p, _p]),
-    "meep2b_head_norm_rotate_backward": (ctypes.c_int, [_p, _p]),
+    "meep2b_head_norm_rotate": (ctypes.c_int, [ctypes.POINTER(HeadNorm), _p]),
+    "meep2b_head_norm_rotate_backward": (ctypes.c_int, [ctypes.POINTER(HeadNorm), _p]),
     "meep2b_linear_ce_plan": (ctypes.c_int, [_i64, _i64, _i64, ctypes.POINTER(_i64), ctypes.POINTER(_i64),
                                              ctypes.POINTER(_i32)]),
-    "meep2b_linear_ce_forward": (ctypes.c_int, [_p, _p]),
-    "meep2b_linear_ce_backward": (ctypes.c_int, [_p, _p]),
+    "meep2b_linear_ce_forward": (ctypes.c_int, [ctypes.POINTER(LinearCE), _p]),
+    "meep2b_linear_ce_backward": (ctypes.c_int, [ctypes.POINTER(LinearCE), _p]),
 }
 
 _lib = None
@@ -169,6 +159,23 @@ def load():
     return lib
 
 
+_native = None
+
+
+def native():
+    """The compiled autograd nodes of the fine-tuning operators (csrc/native.cpp), which call libmeep2b."""
+    global _native
+    if _native is None:
+        load()
+        try:
+            from . import _native as module
+        except ImportError as exc:
+            raise RuntimeError(f"_native.so is not built or does not load ({exc}); run `python -m "
+                               "meepsquared_b200.build`") from exc
+        _native = module
+    return _native
+
+
 def loaded() -> bool:
     try:
         load()
@@ -185,8 +192,8 @@ class DeviceError(RuntimeError):
     pass
 
 
-# Kernels each entry point launches per successful call (the ones this package calls on its hot path), for the
-# count of the library's launches in a timed region (benchmark); `launches` accumulates them per entry point.
+# Kernels each entry point launches per successful call (the ones this package calls through ctypes on its hot path),
+# for the count of the library's launches in a timed region (benchmark); `launches` accumulates them per entry point.
 KERNELS_PER_CALL = {
     "meep2b_route": 3, "meep2b_route_noalloc": 3, "meep2b_route_logits": 3, "meep2b_routed_rows": 1, "meep2b_gather": 1,
     "meep2b_unpermute": 1, "meep2b_unpermute_backward": 1, "meep2b_tile_map": 1, "meep2b_grouped_product": 1,
@@ -196,10 +203,6 @@ KERNELS_PER_CALL = {
     "meep2b_merge_stack": 1,
     "meep2b_quant_multipliers": 1, "meep2b_fp8_rows_quantize": 1, "meep2b_grouped_product_f8": 1,
     "meep2b_swiglu": 1, "meep2b_swiglu_backward": 1, "meep2b_weight_grad": 1, "meep2b_combine": 1,
-    "meep2b_balance_loss": 2, "meep2b_balance_loss_backward": 1,
-    # at least: one more per vocabulary piece and gradient, and with the weights' gradients
-    "meep2b_linear_ce_plan": 0, "meep2b_linear_ce_forward": 4, "meep2b_linear_ce_backward": 1,
-    "meep2b_head_norm_rotate": 1, "meep2b_head_norm_rotate_backward": 1,
 }
 launches = {}
 
@@ -222,12 +225,6 @@ def check(status: int, what: str):
     if status == ERR_UNSUPPORTED:
         raise NotImplementedError(msg)
     raise RuntimeError(msg)
-
-
-def once(backward):
-    """A Function's backward that is not differentiable itself. torch's own wrapper is put around it only where a second
-    derivative could be asked for (grad mode is on in the backward pass); it takes as long as a small kernel."""
-    return torch.autograd.function.once_differentiable(backward) if torch.is_grad_enabled() else backward
 
 
 def ptr(t):

@@ -7,118 +7,13 @@ head that is trained too has its logits computed again in the backward call, sin
 log-sums have to be known first.
 """
 
-import ctypes
-import functools
-
 import torch
 
 from . import _lib
 
 _REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}  # enum meep2b_reduction
-_pack = _lib.packer(_lib.LinearCE).pack
-
-
-@functools.lru_cache(maxsize=256)
-def _plan(tokens, hidden_size, vocab):
-    rows_pad, piece_cols, planes = ctypes.c_int64(), ctypes.c_int64(), ctypes.c_int32()
-    _lib.check(_lib.load().meep2b_linear_ce_plan(tokens, hidden_size, vocab, ctypes.byref(rows_pad),
-                                                 ctypes.byref(piece_cols), ctypes.byref(planes)),
-               "meep2b_linear_ce_plan")
-    return rows_pad.value, piece_cols.value, planes.value
-
-
-def _rows(t):
-    """A 2-D tensor as rows that TMA and 16-byte loads can address: itself, or a copy."""
-    ld, inner = t.stride()
-    if inner == 1 and ld % 8 == 0 and ld >= t.shape[1] and t.data_ptr() % 16 == 0:
-        return t
-    return t.clone(memory_format=torch.contiguous_format)
-
-
-def _call(what, weight, targets, ignore_index, reduction, plan, piece_cols, kept, hidden=0, ld_hidden=0, compact=0,
-          acc=0, piece=0, part=0, row_loss=0, loss=0, upstream=0, d_hidden=0, d_weight=0):
-    rows_pad, _, planes = plan
-    vocab, size = weight.shape
-    # what the passes keep of every row: state (8), flags (rows_pad / 256), source, slot, target and the row values
-    state = kept.data_ptr()
-    source = state + 4 * (8 + rows_pad // 256)
-    step = 4 * rows_pad
-    args = _pack(hidden, targets.numel(), size, ld_hidden, weight.data_ptr(), vocab, weight.stride(0),
-                 targets.data_ptr(), ignore_index, _REDUCTIONS[reduction], planes, rows_pad, piece_cols, state, state + 32,
-                 source, source + step, source + 2 * step, source + 3 * step, compact, acc, piece, part, row_loss, loss,
-                 upstream, d_hidden, d_weight)
-    _lib.check(getattr(_lib.load(), what)(args, _lib.stream_of(weight)), what)
-
-
-def _bytes(sizes, device):
-    """One buffer for all of these sizes, and the address of each (256 bytes apart at least)."""
-    at, ends = 0, []
-    for n in sizes:
-        ends.append(at)
-        at += (n + 255) & ~255
-    buffer = torch.empty(at, dtype=torch.uint8, device=device)
-    base = buffer.data_ptr()
-    return buffer, [base + e for e in ends]
-
-
-def _forward(hidden, weight, targets, ignore_index, reduction, accumulate, keep_rows):
-    """The loss, and what the backward pass needs: the rows' values, with `accumulate` the planes of the hidden states'
-    gradient, with `keep_rows` the copied rows."""
-    tokens, size = hidden.shape
-    vocab = weight.shape[0]
-    dev = hidden.device
-    plan = rows_pad, piece_cols, planes = _plan(tokens, size, vocab)
-    kept = torch.empty(8 + rows_pad // 256 + 8 * rows_pad, dtype=torch.int32, device=dev)
-    loss = torch.empty(tokens if reduction == "none" else (), dtype=torch.float32, device=dev)
-    slots = 2 * ((vocab + 255) // 256)
-    rows = torch.empty((rows_pad, size), dtype=torch.bfloat16, device=dev) if keep_rows else None
-    acc = torch.empty((planes, rows_pad, size), dtype=torch.float32, device=dev) if accumulate else None
-    scratch, (part, row_loss, compact, piece) = _bytes(
-        (4 * slots * rows_pad, 4 * rows_pad, 0 if keep_rows else 2 * rows_pad * size,
-         2 * rows_pad * piece_cols if accumulate else 0), dev)
-    _call("meep2b_linear_ce_forward", weight, targets, ignore_index, reduction, plan, piece_cols if accumulate else 0,
-          kept, hidden=hidden.data_ptr(), ld_hidden=hidden.stride(0),
-          compact=rows.data_ptr() if keep_rows else compact, acc=acc.data_ptr() if accumulate else 0,
-          piece=piece if accumulate else 0, part=part, row_loss=row_loss, loss=loss.data_ptr())
-    return loss, kept, rows, acc, plan
-
-
-def _backward(ctx, grad):
-    weight, targets, kept, last = ctx.saved_tensors
-    need_hidden, need_weight = ctx.needs_input_grad[:2]
-    w = _rows(weight)
-    vocab, size = w.shape
-    rows_pad, piece_cols, planes = ctx.plan
-    upstream = grad.to(torch.float32).contiguous()
-    d_hidden = w.new_empty((targets.numel(), size)) if need_hidden else None
-    d_weight = None
-    where = dict(upstream=upstream.data_ptr(), d_hidden=d_hidden.data_ptr() if need_hidden else 0)
-    if need_weight:
-        d_weight = w.new_empty((vocab, size))
-        scratch, (piece, acc) = _bytes((2 * rows_pad * piece_cols, 4 * planes * rows_pad * size if need_hidden else 0),
-                                       w.device)
-        where.update(piece=piece, acc=acc if need_hidden else 0, compact=last.data_ptr(), d_weight=d_weight.data_ptr())
-    else:
-        where.update(acc=last.data_ptr())
-    _call("meep2b_linear_ce_backward", w, targets, ctx.ignore_index, ctx.reduction, ctx.plan, piece_cols, kept, **where)
-    return d_hidden, d_weight, None, None, None
-
-
-class _LinearCrossEntropy(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, hidden, weight, targets, ignore_index, reduction):
-        train_head = ctx.needs_input_grad[1]
-        accumulate = ctx.needs_input_grad[0] and not train_head
-        loss, kept, rows, acc, ctx.plan = _forward(_rows(hidden), _rows(weight), targets, ignore_index, reduction,
-                                                   accumulate, train_head)
-        # of the hidden states the backward pass reads the copied rows, and those with a trained head alone
-        ctx.save_for_backward(weight, targets, kept, rows if train_head else acc)
-        ctx.reduction, ctx.ignore_index = reduction, ignore_index
-        return loss
-
-    @staticmethod
-    def backward(ctx, grad):
-        return _lib.once(_backward)(ctx, grad)
+# columns of a vocabulary piece (a multiple of 256) and planes of the gradient's sums; 0: as meep2b_linear_ce_plan says
+PLAN = (0, 0)
 
 
 def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, ignore_index: int = -100,
@@ -153,8 +48,5 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
     if t.numel() == 0:  # nothing to compute; the graph is kept
         zero = (hidden.sum(dtype=torch.float32) + weight[:0].sum(dtype=torch.float32))
         return zero + hidden.new_zeros(targets.shape, dtype=torch.float32) if reduction == "none" else zero
-    if torch.is_grad_enabled() and (flat.requires_grad or weight.requires_grad):
-        loss = _LinearCrossEntropy.apply(flat, weight, t, ignore_index, reduction)
-    else:
-        loss = _forward(_rows(flat.detach()), _rows(weight.detach()), t, ignore_index, reduction, False, False)[0]
+    loss = _lib.native().linear_cross_entropy(flat, weight, t, ignore_index, _REDUCTIONS[reduction], *PLAN)
     return loss.view(targets.shape) if reduction == "none" else loss

@@ -1,4 +1,5 @@
-"""Builds libmeep2b.so in the package directory with nvcc for sm_100a (B200) only.
+"""Builds libmeep2b.so in the package directory with nvcc for sm_100a (B200) only, and _native.so, the autograd nodes that
+call it, with the host compiler against the installed torch.
 
     python -m meepsquared_b200.build [--verbose]
 
@@ -10,6 +11,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB = os.path.join(HERE, "libmeep2b.so")
@@ -17,6 +19,10 @@ SOURCES = ["libmeep2b.cu", "capi.cu", "route.cu", "grouped_gemm.cu", "grouped_ge
            "reduce.cu", "quant.cu", "merge.cu", "fp8_products.cu", "swiglu.cu", "vocab_loss.cu",
            "balance.cu", "head_norm.cu",
            "common.cuh", "host.hpp"]
+
+
+NATIVE = os.path.join(HERE, "_native.so")
+NATIVE_SOURCE = os.path.join(HERE, "csrc", "native.cpp")
 
 
 def nvcc() -> str:
@@ -35,8 +41,42 @@ def stale() -> bool:
 
 
 def build(verbose: bool = False, force: bool = False) -> str:
-    if not force and not stale():
-        return LIB
+    if force or stale():
+        build_library(verbose)
+    if force or native_stale():
+        build_native(verbose)
+    return LIB
+
+
+def native_stale() -> bool:
+    if not os.path.exists(NATIVE):
+        return True
+    t = os.path.getmtime(NATIVE)
+    return any(os.path.getmtime(d) > t for d in (NATIVE_SOURCE, os.path.join(HERE, "..", "include", "meep2b.h")))
+
+
+def build_native(verbose: bool = False) -> str:
+    import torch
+
+    cxx = os.environ.get("CXX") or shutil.which("g++") or "c++"
+    root = os.path.dirname(torch.__file__)
+    cuda = os.path.dirname(os.path.dirname(os.path.realpath(nvcc())))
+    includes = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
+                sysconfig.get_paths()["include"], os.path.join(cuda, "include")]
+    cmd = [cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-DTORCH_EXTENSION_NAME=_native",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *[f"-I{d}" for d in includes], NATIVE_SOURCE,
+           "-o", NATIVE + ".tmp", f"-L{HERE}", "-l:" + os.path.basename(LIB), "-L" + os.path.join(root, "lib"), "-lc10",
+           "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError("the host compiler failed:\n" + r.stdout + r.stderr)
+    if verbose:
+        sys.stderr.write(r.stdout + r.stderr)
+    os.replace(NATIVE + ".tmp", NATIVE)
+    return NATIVE
+
+
+def build_library(verbose: bool = False) -> str:
     cmd = [nvcc(), "-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std=c++17",
            "--expt-relaxed-constexpr", "-Xcompiler", "-fPIC", "-shared", "-cudart", "static",
            "-o", LIB + ".tmp", os.path.join(HERE, "csrc", "libmeep2b.cu")]

@@ -7,14 +7,21 @@ import pytest
 import torch
 
 import meepsquared_b200 as mb
-from meepsquared_b200 import _lib, _loss
+from meepsquared_b200 import _lib, build
+
+
+def plan(tokens, hidden, vocab):
+    rows, cols, planes = ctypes.c_int64(), ctypes.c_int64(), ctypes.c_int32()
+    _lib.check(_lib.load().meep2b_linear_ce_plan(tokens, hidden, vocab, ctypes.byref(rows), ctypes.byref(cols),
+                                                 ctypes.byref(planes)), "meep2b_linear_ce_plan")
+    return rows.value, cols.value, planes.value
 
 
 @pytest.mark.parametrize("tokens", [1, 255, 256, 257, 4096, 16384, 1 << 20])
 @pytest.mark.parametrize("vocab", [1, 256, 257, 32003, 131072, 262144])
 @pytest.mark.parametrize("hidden", [8, 2048, 8192])
 def test_the_plan_of_the_vocabulary_loss(tokens, vocab, hidden):
-    rows, cols, planes = _loss._plan(tokens, hidden, vocab)
+    rows, cols, planes = plan(tokens, hidden, vocab)
     assert rows % 256 == 0 and tokens <= rows < tokens + 256
     assert cols % 256 == 0 and 256 <= cols < vocab + 256
     assert cols == 256 or rows * cols * 2 <= 1 << 30
@@ -25,24 +32,15 @@ def test_the_plan_of_the_vocabulary_loss(tokens, vocab, hidden):
 
 def test_sizes_beyond_the_entry_point_are_refused():
     with pytest.raises(ValueError):
-        _loss._plan(1 << 25, 64, 1000)
+        plan(1 << 25, 64, 1000)
     with pytest.raises(ValueError):
-        _loss._plan(16, 0, 1000)
+        plan(16, 0, 1000)
 
 
-@pytest.mark.parametrize("cls", [_lib.Balance, _lib.HeadNorm, _lib.LinearCE])
-def test_packed_arguments_are_the_structures_bytes(cls):
-    pack = _lib.packer(cls)
-    values, n = [], 1
-    filled = cls()
-    for name, kind in cls._fields_:
-        count = getattr(kind, "_length_", 1)
-        some = [float(n + i) if kind is ctypes.c_float else n + i for i in range(count)]
-        setattr(filled, name, kind(*some) if count > 1 else some[0])
-        values += some
-        n += count
-    got = pack.pack(*values)
-    assert got == bytes(filled)[:len(got)] and not any(bytes(filled)[len(got):])
+def test_the_autograd_nodes_build_and_load():
+    build.build()
+    module = _lib.native()
+    assert all(callable(getattr(module, f)) for f in ("linear_cross_entropy", "balance_loss", "qk_norm_rope"))
 
 
 def test_no_cpu_fallback():

@@ -180,6 +180,22 @@ def test_other_strides_streams_and_again():
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
 
 
+def test_a_second_derivative_is_refused():
+    xs = [x.requires_grad_() for x in make(2, 20, 16, torch.float32)]
+    grads = torch.autograd.grad(mb.balance_loss(xs, 2)[0], xs, create_graph=True)
+    with pytest.raises(RuntimeError, match="not differentiable twice"):
+        grads[0].sum().backward()
+
+
+def test_some_layers_gradients_alone():
+    xs = make(3, 20, 16, torch.float32)
+    want = [x.detach().requires_grad_() for x in xs]
+    mb.balance_loss(want, 2)[0].backward()
+    some = [x.detach().requires_grad_(i != 1) for i, x in enumerate(xs)]
+    mb.balance_loss(some, 2)[0].backward()
+    assert some[1].grad is None and all(torch.equal(some[i].grad, want[i].grad) for i in (0, 2))
+
+
 def test_refusals():
     x = make(1, 10, 16, torch.float32)[0]
     with pytest.raises(ValueError, match="top_k"):

@@ -237,6 +237,26 @@ def test_again_on_another_stream_and_empty():
     assert out[0].shape[0] == 0 and not grads[2].any() and not grads[3].any()
 
 
+def test_a_second_derivative_is_refused():
+    q, k, wq, wk, dq, dk = make(1, 8, 2, 1, 64, torch.float32)
+    cos, sin = angles(8, 32)
+    q.requires_grad_()
+    grad, = torch.autograd.grad(mb.qk_norm_rope(q, k, wq, wk, cos, sin), q, [dq, dk], create_graph=True)
+    with pytest.raises(RuntimeError, match="not differentiable twice"):
+        grad.sum().backward()
+
+
+def test_an_input_changed_in_place_is_noticed():
+    q, k, wq, wk, dq, dk = make(1, 8, 2, 1, 64, torch.float32)
+    cos, sin = angles(8, 32)
+    leaf = q.requires_grad_()
+    x = leaf * 1.0
+    out = mb.qk_norm_rope(x, k, wq, wk, cos, sin)
+    x.mul_(2.0)
+    with pytest.raises(RuntimeError, match="inplace"):
+        torch.autograd.grad(out, leaf, [dq, dk])
+
+
 def test_refusals():
     q, k, wq, wk, _, _ = make(1, 4, 2, 1, 64, torch.bfloat16)
     cos, sin = angles(4, 32)

@@ -131,12 +131,7 @@ def test_what_ignored_tokens_hold_does_not_matter(head):
 @pytest.mark.parametrize("planes", [1, 3, 16])
 @pytest.mark.parametrize("piece_cols", [256, 768])
 def test_pieces_and_planes(monkeypatch, piece_cols, planes, head):
-    plan = _loss._plan
-
-    def small(tokens, size, vocab):
-        return plan(tokens, size, vocab)[0], piece_cols, planes
-
-    monkeypatch.setattr(_loss, "_plan", small)
+    monkeypatch.setattr(_loss, "PLAN", (piece_cols, planes))
     h, w, t = inputs(600, 192, 2000, ignored=0.2)
     check(h, w, t, "none", head)
 
@@ -147,8 +142,7 @@ def test_targets_far_below_the_largest_logit(monkeypatch, pieces, hidden):
     """Logits hundreds above the target's: beyond the window of the target's own reference, in some rows of some
     tiles (the others keep theirs), and far below it."""
     if pieces:
-        plan = _loss._plan
-        monkeypatch.setattr(_loss, "_plan", lambda *a: (plan(*a)[0], 512, 2))
+        monkeypatch.setattr(_loss, "PLAN", (512, 2))
     h, w, t = inputs(700, hidden, 1500)
     far = torch.arange(700, device=DEV) % 97 == 5
     h[far] *= 200.0   # logits of +-600 or so
@@ -258,6 +252,19 @@ def test_again_and_on_another_stream():
         if first is None:
             first = got
         assert all(torch.equal(x, y) for x, y in zip(first, got))
+
+
+@pytest.mark.parametrize("head", [False, True], ids=["frozen", "trained"])
+def test_a_second_derivative_is_refused(head):
+    h, w, t = inputs(20, 64, 70)
+    h, w = h.requires_grad_(), w.requires_grad_(head)
+    grad, = torch.autograd.grad(mb.linear_cross_entropy(h, w, t), h, create_graph=True)
+    with pytest.raises(RuntimeError, match="not differentiable twice"):
+        grad.float().sum().backward()
+    loss = mb.linear_cross_entropy(h, w, t)
+    loss.backward()
+    with pytest.raises(RuntimeError, match="second time"):
+        loss.backward()
 
 
 def test_one_gradient_without_the_other():
