@@ -18,7 +18,7 @@
 //
 // The products are one persistent tcgen05 kernel on CTA pairs (M = 256, N = 256, K = 64 a stage, both operands by
 // TMA, two accumulators in tensor memory), with a mode for each epilogue:
-//   kStats    the row sums of a 256-column tile (two 128-column halves), nothing else
+//   kStats    the row sums of a 256-column tile (its two halves), nothing else
 //   kProbs    the same, and q as bf16 into the vocabulary piece's buffer
 //   kReprobs  q alone, for the row tiles to be computed again
 //   kGrad     g (q / Z - [v = y]) as bf16 into the piece's buffer (the head's gradient, and dh beside it)
@@ -39,11 +39,10 @@ constexpr int BK = 64;
 constexpr int STAGES = 6;
 constexpr int OPERAND_BYTES = 128 * BK * 2;  // each CTA's half of A or of B, one stage
 constexpr int STAGE_BYTES = 2 * OPERAND_BYTES;
-constexpr int THREADS = 384;
 constexpr int EPI_WARP0 = 4;
-constexpr int STG_BYTES = 4096;  // per epilogue warp
+constexpr int STG_BYTES = 32768;  // the epilogue warps' tiles on their way out
 constexpr int OFF_STG = STAGES * STAGE_BYTES;
-constexpr int OFF_BAR = OFF_STG + 8 * STG_BYTES;
+constexpr int OFF_BAR = OFF_STG + STG_BYTES;
 constexpr int NUM_BARS = 2 * STAGES + 5;
 constexpr int OFF_TMEM = OFF_BAR + NUM_BARS * 8;
 constexpr int SMEM_BYTES = OFF_TMEM + 16 + 1024;
@@ -57,6 +56,18 @@ constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kWindow = 7.9228162514264338e28f;  // 2^96
 
 enum Mode { kStats, kProbs, kReprobs, kGrad, kAcc, kWeight };
+
+// Epilogue warps, in groups of 8 (four quarters of the rows, which a warp may read of tensor memory, by two halves of the
+// columns). Over the logits every element costs an exponential, and one group, each of whose warps waits for the unit,
+// loads, computes and stores in turn, left the exponentials' unit idle more than half of the time: two groups take every
+// other unit each (5,200 cycles a unit with one, the exponentials alone are 2,048, the product's time at hidden 256).
+// The other modes have time enough with one, and DEEP needs its registers.
+template <int MODE, bool DEEP>
+struct Epi {
+  static constexpr int GROUPS = MODE == kAcc || MODE == kWeight || DEEP ? 1 : 2;
+  static constexpr int THREADS = 32 * (EPI_WARP0 + 8 * GROUPS);
+};
+constexpr int SLOTS = 2;  // row sums kept for a column tile, one for every half
 
 // ints of `state`
 enum { kLive = 0, kRedo = 1, kDone = 2, kParts = 3, kStateInts = 8 };  // (kParts: planes that kAcc wrote)
@@ -75,7 +86,7 @@ struct Params {
   const int32_t* target;   // per live row (-1 past the last)
   const int32_t* source;   // the live row's token
   Rows rows;
-  float* part;             // (2 * column tiles of the vocabulary) x rows_pad: the row sums
+  float* part;             // (SLOTS * column tiles of the vocabulary) x rows_pad: the row sums
   int64_t rows_pad;
   const float* upstream;   // one value, or one per token
   int per_token, mean;     // how g follows from it
@@ -186,144 +197,155 @@ __device__ __forceinline__ float row_upstream(const float* upstream, int per_tok
 // The gradient of the target's own logit, g (p - 1).
 __device__ __forceinline__ float target_gradient(float miss, float g) { return __fmul_rn(-miss, g); }
 
-// One unit's epilogue for one warp: 32 rows (a lane each) and 128 columns, 32 at a time.
-// held (DEEP): the unit's sums, already out of tensor memory.
-template <int MODE, bool DEEP>
-__device__ __forceinline__ void epilogue(const Params& p, const CUtensorMap* out, int m, int n, int part, bool empty,
-                                         int row0, int half, uint32_t acc, int lane, uint32_t stg, uint32_t tempty,
-                                         int live, float (&held)[4][32]) {
-  const int row = row0 + lane;  // of the live rows (kWeight: of the piece's columns)
-  constexpr bool LOGITS = MODE == kStats || MODE == kProbs || MODE == kReprobs || MODE == kGrad;
-  const int c_first = n * TILE + half * 128;  // column of the product
+// 32 columns of the warp's rows of an accumulator, on their way (load) and there (the registers named, so that they are
+// read only afterwards).
+__device__ __forceinline__ void tmem_load32(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_loaded(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                 "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]),
+                 "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
+                 "+r"(r[30]), "+r"(r[31])
+               :
+               : "memory");
+}
+
+// What an epilogue thread knows of its row of a unit before the unit's sums arrive.
+struct RowIn {
   float ref = 0.f, g = 0.f, miss = 0.f;
   int target = -1;
-  if (LOGITS) {
-    target = p.target[row];
-    ref = MODE == kGrad ? p.rows.lse[row] : p.rows.ref[row];
-    if (MODE == kGrad && row < live) {
-      g = row_upstream(p.upstream, p.per_token, p.mean, p.source[row], live);
-      miss = p.rows.miss[row];
-    }
+};
+
+template <int MODE>
+__device__ __forceinline__ RowIn row_in(const Params& p, int row, int live) {
+  RowIn r;
+  if (MODE == kAcc || MODE == kWeight || row >= live) return r;
+  r.target = p.target[row];
+  r.ref = MODE == kGrad ? p.rows.lse[row] : p.rows.ref[row];
+  if (MODE == kGrad) {
+    r.g = row_upstream(p.upstream, p.per_token, p.mean, p.source[row], live);
+    r.miss = p.rows.miss[row];
   }
-  float sum = 0.f, far = -INFINITY;  // the sum within the window; log2 of what lies above it, against the reference
-#pragma unroll(DEEP ? 4 : 1)
-  for (int c = 0; c < 4; ++c) {
-    const int col = c_first + 32 * c;
-    float v[32];
-    if (DEEP) {
+  return r;
+}
+
+// The sums over the vocabulary of one row of a unit: what lies within the window, and log2 of what lies above it,
+// against the reference.
+struct RowSums {
+  float sum = 0.f, far = -INFINITY;
+};
+
+// 32 columns of a unit from column `col` of the product, a lane a row (the first is row0): to q, to g (q - [v = y]), or
+// as they are, into shared memory and from there out by TMA; and the row's sums.
+template <int MODE, int TILES>
+__device__ __forceinline__ void columns32(const Params& p, const CUtensorMap* out, const RowIn& in, RowSums& sums,
+                                          float (&v)[32], int c, int col, int part, bool empty, int row0, int live,
+                                          int lane, uint32_t stg) {
+  constexpr bool LOGITS = MODE == kStats || MODE == kProbs || MODE == kReprobs || MODE == kGrad;
+  const int row = row0 + lane;  // of the live rows (kWeight: of the piece's columns)
+  const int vcol = p.v0 + col;  // LOGITS: of the vocabulary
+  const bool own = in.target >= vcol && in.target < vcol + 32;
+  if (LOGITS) {
+    if (vcol + 32 > p.vocab || own) {  // past the end, or the target's own
 #pragma unroll
-      for (int j = 0; j < 32; ++j) v[j] = held[c][j];
-    } else {
-      tmem_ld32(acc + 32 * c, v);
-      if (c == 3) {
-        tc_fence_before();
-        mbar_arrive_remote(tempty, 0);  // the whole accumulator has been read
+      for (int j = 0; j < 32; ++j)
+        if (vcol + j >= p.vocab || vcol + j == in.target) v[j] = -INFINITY;
+    }
+    float e[32];
+#pragma unroll
+    for (int j = 0; j < 32; ++j) e[j] = exp2_fast(fmaf(v[j], kLog2e, -in.ref));
+    if (MODE == kStats || MODE == kProbs) {
+      float s[4] = {e[0], e[1], e[2], e[3]};
+#pragma unroll
+      for (int j = 4; j < 32; ++j) s[j & 3] += e[j];
+      const float all = (s[0] + s[1]) + (s[2] + s[3]);
+      if (all < kWindow || row >= live) {
+        sums.sum += all;
+      } else {  // against the columns' own maximum (a NaN stays one)
+        float top = v[0];
+#pragma unroll
+        for (int j = 1; j < 32; ++j) top = fmaxf(top, v[j]);
+        float t = 0.f;
+#pragma unroll
+        for (int j = 0; j < 32; ++j) t += exp2_fast((v[j] - top) * kLog2e);
+        const float here = fmaf(top, kLog2e, -in.ref) + log2f(t);
+        const float hi = fmaxf(sums.far, here), lo = fminf(sums.far, here);
+        sums.far = here != here ? here : (sums.far != sums.far ? sums.far : hi + log2f(1.0f + exp2f(lo - hi)));
       }
     }
-    if (LOGITS) {
-      const int vcol = p.v0 + col;  // of the vocabulary
-      if (vcol + 32 > p.vocab || (target >= vcol && target < vcol + 32)) {  // past the end, or the target's own
+    if (MODE == kStats) return;
+    if (MODE == kGrad) {  // (rows past the last live one are zero: the head's gradient sums over them)
+#pragma unroll
+      for (int j = 0; j < 32; ++j) e[j] = row < live ? e[j] * in.g : 0.f;
+      if (own) {
 #pragma unroll
         for (int j = 0; j < 32; ++j)
-          if (vcol + j >= p.vocab || vcol + j == target) v[j] = -INFINITY;
-      }
-      float e[32];
-      float s = 0.f;
-#pragma unroll
-      for (int j = 0; j < 32; ++j) {
-        e[j] = exp2_fast(fmaf(v[j], kLog2e, -ref));
-        s += e[j];
-      }
-      if (MODE == kStats || MODE == kProbs) {
-        if (s < kWindow) {
-          sum += s;
-        } else {  // against the piece's own maximum (a NaN stays one)
-          float top = v[0];
-#pragma unroll
-          for (int j = 1; j < 32; ++j) top = fmaxf(top, v[j]);
-          float t = 0.f;
-#pragma unroll
-          for (int j = 0; j < 32; ++j) t += exp2_fast((v[j] - top) * kLog2e);
-          const float here = fmaf(top, kLog2e, -ref) + log2f(t);
-          const float hi = fmaxf(far, here), lo = fminf(far, here);
-          far = here != here ? here : (far != far ? far : hi + log2f(1.0f + exp2f(lo - hi)));
-        }
-      }
-      if (MODE == kGrad) {  // (rows past the last live one are zero: the head's gradient sums over them)
-#pragma unroll
-        for (int j = 0; j < 32; ++j) e[j] = row < live ? e[j] * g : 0.f;
-        if (target >= vcol && target < vcol + 32) {
-#pragma unroll
-          for (int j = 0; j < 32; ++j)
-            if (vcol + j == target) e[j] = target_gradient(miss, g);
-        }
-      }
-      if (MODE != kStats) {
-        uint32_t w[16];
-#pragma unroll
-        for (int j = 0; j < 16; ++j) w[j] = pack_bf16x2(e[2 * j], e[2 * j + 1]);
-        const uint32_t tile = stg + (c & 1) * 2048u;
-        if (lane == 0) bulk_wait_read<1>();  // the tile's last store has read it
-        __syncwarp();
-        stage_bf16(tile, lane, w);
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) {
-          tma_store_2d(out, tile, col, row0);
-          bulk_commit();
-        }
-      }
-    } else {
-      if (empty) {
-#pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] = 0.f;
-      }
-      if (MODE == kAcc) {
-        if (lane == 0) bulk_wait_read<0>();
-        __syncwarp();
-        stage_f32(stg, lane, v);
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0 && col < p.hidden) {
-          const int at = part * static_cast<int>(p.rows_pad) + row0;
-          if (p.first)
-            tma_store_2d(out, stg, col, at);
-          else
-            tma_add_2d(out, stg, col, at);
-          bulk_commit();
-        }
-      } else {
-        uint32_t w[16];
-#pragma unroll
-        for (int j = 0; j < 16; ++j) w[j] = pack_bf16x2(v[2 * j], v[2 * j + 1]);
-        const uint32_t tile = stg + (c & 1) * 2048u;
-        if (lane == 0) bulk_wait_read<1>();
-        __syncwarp();
-        stage_bf16(tile, lane, w);
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) {
-          if (col < p.hidden && p.v0 + row0 < p.vocab) tma_store_2d(out, tile, col, p.v0 + row0);
-          bulk_commit();
-        }
+          if (vcol + j == in.target) e[j] = target_gradient(in.miss, in.g);
       }
     }
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] = e[j];
+  } else if (empty) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] = 0.f;
   }
-  if (MODE == kStats || MODE == kProbs) {
-    const int slot = 2 * (p.v0 / TILE + n) + half;
-    // what lies above the window is kept as minus its log2 against the reference (over 90, so never near zero)
-    float kept = sum;
-    if (far != -INFINITY) kept = far != far ? far : -(far + log2f(1.0f + sum * exp2f(-far)));
-    p.part[static_cast<int64_t>(slot) * p.rows_pad + row] = kept;
+  if (MODE == kAcc) {
+    if (lane == 0) bulk_wait_read<0>();  // the tile's last store has read it
+    __syncwarp();
+    stage_f32(stg, lane, v);
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0 && col < p.hidden) {
+      const int at = part * static_cast<int>(p.rows_pad) + row0;
+      if (p.first)
+        tma_store_2d(out, stg, col, at);
+      else
+        tma_add_2d(out, stg, col, at);
+      bulk_commit();
+    }
+  } else {
+    uint32_t w[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) w[j] = pack_bf16x2(v[2 * j], v[2 * j + 1]);
+    // two tiles a warp of one group, one of two
+    const uint32_t tile = stg + (TILES == 2 ? (c & 1) * 2048u : 0u);
+    if (lane == 0) bulk_wait_read<TILES - 1>();
+    __syncwarp();
+    stage_bf16(tile, lane, w);
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+      if (LOGITS || (col < p.hidden && p.v0 + row0 < p.vocab)) tma_store_2d(out, tile, col, LOGITS ? row0 : p.v0 + row0);
+      bulk_commit();
+    }
   }
 }
 
+// A row's sums over half a unit's columns, kept for the join: what lies above the window as minus its log2 against the
+// reference (over 90, so never near zero).
+__device__ __forceinline__ void keep_sums(const Params& p, const RowSums& s, int n, int half, int row) {
+  float kept = s.sum;
+  if (s.far != -INFINITY) kept = s.far != s.far ? s.far : -(s.far + log2f(1.0f + s.sum * exp2f(-s.far)));
+  p.part[static_cast<int64_t>(SLOTS * (p.v0 / TILE + n) + half) * p.rows_pad + row] = kept;
+}
+
 template <int MODE, bool REDO, bool DEEP>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__((Epi<MODE, DEEP>::THREADS), 1)
     vocab_product(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap ta32,
                   const __grid_constant__ CUtensorMap tb, const __grid_constant__ CUtensorMap tout, const Params p) {
   constexpr bool A_MN = MODE == kWeight;
   constexpr bool B_MN = MODE == kWeight || MODE == kAcc;
+  using E = Epi<MODE, DEEP>;
   if (REDO) {
     let_next_start();
     wait_for_last();
@@ -351,7 +373,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(bar_tfull(b), 1);
-      mbar_init(bar_tempty(b), 512);  // 256 epilogue threads of each CTA
+      mbar_init(bar_tempty(b), 16);  // eight epilogue warps of each CTA
     }
     mbar_init(bar_drain, 1);
     fence_barrier_init();
@@ -471,48 +493,93 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     }
   } else {  // ------------------------------------------------------------------------------- epilogue (each CTA)
     if (DEEP) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
-    const int q = warp & 3, half = (warp - EPI_WARP0) >> 2;
-    const uint32_t stg = sbase + OFF_STG + static_cast<uint32_t>(warp - EPI_WARP0) * STG_BYTES;
-    int it = 0;
-    for (int u = pair_id; u < w.total; u += pairs) {
-      int m, n, part;
-      w.decode(u, m, n, part);
-      if (REDO && p.flags[m] == 0) continue;
-      float held[4][32];
-      if (DEEP) {
-        const int passes = (w.kblocks + DEEP_BLOCKS - 1) / DEEP_BLOCKS;
-        bool ok = true;
+    const int q = warp & 3, half = ((warp - EPI_WARP0) >> 2) & 1, group = (warp - EPI_WARP0) >> 3;
+    const uint32_t stg = sbase + OFF_STG + static_cast<uint32_t>(warp - EPI_WARP0) * (STG_BYTES / (8 * E::GROUPS));
+    auto release = [&](uint32_t bar) {  // the warp is done with an accumulator: one arrival for its 32 lanes
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_remote(bar, 0);
+    };
+    // the next unit, and what is known of this thread's row in it, are looked up a unit ahead
+    const int row_in_tile = 128 * static_cast<int>(rank) + 32 * q;
+    // (computing again, units without a flag are passed over, and the groups alternate over what remains)
+    const int first = REDO ? pair_id : pair_id + group * pairs, step = REDO ? pairs : E::GROUPS * pairs;
+    int it = REDO ? 0 : group, m = 0, n = 0, part = 0;
+    RowIn next;
+    if (first < w.total) {
+      w.decode(first, m, n, part);
+      next = row_in<MODE>(p, m * TILE + row_in_tile + lane, live);
+    }
+    for (int u = first; u < w.total; u += step) {
+      const int row0 = m * TILE + row_in_tile, c_first = n * TILE + half * 128, tile_n = n, tile_m = m, my_part = part;
+      const RowIn in = next;
+      if (u + step < w.total) {
+        w.decode(u + step, m, n, part);
+        next = row_in<MODE>(p, m * TILE + row_in_tile + lane, live);
+      }
+      if (REDO) {
+        if (p.flags[tile_m] == 0) continue;
+        if (E::GROUPS == 2 && (it & 1) != group) {
+          ++it;
+          continue;
+        }
+      }
+      // a warp without live rows has nothing to write (kGrad: but zeros, to the end of the last k-block of 64 rows)
+      const bool idle = MODE == kWeight ? false : MODE == kGrad ? row0 >= (live + BK - 1) / BK * BK : row0 >= live;
+      const bool empty = w.k_begin(my_part) == w.k_begin(my_part + 1);
+      const int passes = DEEP ? (w.kblocks + DEEP_BLOCKS - 1) / DEEP_BLOCKS : 1;
+      float held[DEEP ? 4 : 1][32];
 #pragma unroll
-        for (int c = 0; c < 128; ++c) held[c / 32][c % 32] = 0.f;
-        for (int pass = 0; pass < passes; ++pass, ++it) {
-          const int ab = it & 1;
-          ok = mbar_wait(bar_tfull(ab), (it >> 1) & 1);
-          if (!ok) break;
-          tc_fence_after();
-          const uint32_t acc = tmem_base + ab * TILE + half * 128 + (static_cast<uint32_t>(32 * q) << 16);
+      for (int c = 0; c < (DEEP ? 128 : 0); ++c) held[c / 32][c % 32] = 0.f;
+      RowSums sums;
+      bool ok = true;
+      for (int pass = 0; pass < passes; ++pass, it += REDO ? 1 : E::GROUPS) {
+        const int ab = it & 1;
+        ok = mbar_wait(bar_tfull(ab), (it >> 1) & 1);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t acc = tmem_base + ab * TILE + half * 128 + (static_cast<uint32_t>(32 * q) << 16);
+        if (idle) {
+          release(bar_tempty(ab));
+          continue;
+        }
+        if (DEEP) {
 #pragma unroll
           for (int c = 0; c < 8; ++c) {
             float v[16];
             tmem_ld16(acc + 16 * c, v);
 #pragma unroll
-            for (int j = 0; j < 16; ++j) held[c / 2][16 * (c % 2) + j] += v[j];
+            for (int j = 0; j < 16; ++j) held[DEEP ? c / 2 : 0][16 * (c % 2) + j] += v[j];
           }
-          tc_fence_before();
-          mbar_arrive_remote(bar_tempty(ab), 0);
+          release(bar_tempty(ab));
+        } else {
+          // the next 32 columns are on their way while these are worked on, where registers allow (one group)
+          constexpr int BUFFERS = E::GROUPS == 1 ? 2 : 1;
+          uint32_t r[BUFFERS][32];
+          tmem_load32(acc, r[0]);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            if (BUFFERS == 1 && c > 0) tmem_load32(acc + 32 * c, r[0]);
+            tmem_loaded(r[c % BUFFERS]);
+            if (BUFFERS == 2 && c < 3) tmem_load32(acc + 32 * (c + 1), r[(c + 1) % BUFFERS]);
+            if (c == 3) release(bar_tempty(ab));  // the whole accumulator has been read
+            float v[32];
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[c % BUFFERS][j]);
+            columns32<MODE, E::GROUPS == 1 ? 2 : 1>(p, &tout, in, sums, v, c, c_first + 32 * c, my_part, empty, row0, live,
+                                                   lane, stg);
+          }
         }
-        if (!ok) break;
-        epilogue<MODE, DEEP>(p, &tout, m, n, part, false, m * TILE + 128 * static_cast<int>(rank) + 32 * q, half, 0u,
-                             lane, stg, 0u, live, held);
-        continue;
       }
-      const int ab = it & 1;
-      if (!mbar_wait(bar_tfull(ab), (it >> 1) & 1)) break;
-      tc_fence_after();
-      const uint32_t acc = tmem_base + ab * TILE + half * 128 + (static_cast<uint32_t>(32 * q) << 16);
-      epilogue<MODE, DEEP>(p, &tout, m, n, part, w.k_begin(part) == w.k_begin(part + 1),
-                           m * TILE + 128 * static_cast<int>(rank) + 32 * q, half, acc, lane, stg, bar_tempty(ab), live,
-                           held);
-      ++it;
+      if (!ok) break;
+      if (idle) continue;
+      if (DEEP) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          columns32<MODE, E::GROUPS == 1 ? 2 : 1>(p, &tout, in, sums, held[DEEP ? c : 0], c, c_first + 32 * c, my_part,
+                                                  empty, row0, live, lane, stg);
+      }
+      if (MODE == kStats || MODE == kProbs) keep_sums(p, sums, tile_n, half, row0 + lane);
     }
     if (lane == 0) bulk_wait_all();
   }
@@ -853,7 +920,7 @@ static int launch_product(const CUtensorMap& a, const CUtensorMap& a32, const CU
     }
     if (device < 64) configured |= uint64_t(1) << device;
   }
-  return launch_chained(after, kern, 2u * pairs, THREADS, SMEM_BYTES, s, a, a32, b, out, p);
+  return launch_chained(after, kern, 2u * pairs, Epi<MODE, DEEP>::THREADS, SMEM_BYTES, s, a, a32, b, out, p);
 }
 
 template <int MODE, bool REDO>
@@ -1007,7 +1074,7 @@ int meep2b_linear_ce_forward(const meep2b_linear_ce* a, void* stream) {
     MEEP2B_TRY(vocab::launch_chained(false, vocab::vocab_scan, 1, 1024, 0, s, a->targets, a->tokens, a->ignore_index,
                                      a->source, a->slot, a->state, a->flags, row_tiles,
                                      per_token ? a->loss : static_cast<float*>(nullptr)));
-  const int slots = 2 * static_cast<int>((a->vocab + vocab::TILE - 1) / vocab::TILE);
+  const int slots = vocab::SLOTS * static_cast<int>((a->vocab + vocab::TILE - 1) / vocab::TILE);
   int pairs = 0;
   MEEP2B_TRY(pairs_of_device(&pairs));
   CeMaps m;
