@@ -17,7 +17,7 @@
 // below), which also keeps what stands in ignored rows, infinities and NaN included, out of every sum.
 //
 // The products are one persistent tcgen05 kernel on CTA pairs (M = 256, N = 256, K = 64 a stage, both operands by
-// TMA, two accumulators in tensor memory), with a mode for each epilogue:
+// TMA, two accumulators in tensor memory), or on single CTAs for few tokens, with a mode for each epilogue:
 //   kStats    the row sums of a 256-column tile (its two halves), nothing else
 //   kProbs    the same, and q as bf16 into the vocabulary piece's buffer
 //   kReprobs  q alone, for the row tiles to be computed again
@@ -36,14 +36,24 @@ namespace vocab {
 
 constexpr int TILE = 256;   // rows and columns of a unit (a CTA pair)
 constexpr int BK = 64;
-constexpr int STAGES = 6;
-constexpr int OPERAND_BYTES = 128 * BK * 2;  // each CTA's half of A or of B, one stage
-constexpr int STAGE_BYTES = 2 * OPERAND_BYTES;
+constexpr int OPERAND_BYTES = 128 * BK * 2;  // 128 rows or columns of an operand, one stage
+constexpr int RING_BYTES = 192 * 1024;
+
+// A unit is 256 rows on a CTA pair, each CTA with its 128 rows and half of the 256 columns; or (SOLO), where a call has
+// no more than 128 tokens, 128 rows on one CTA with all 256 columns: a pair would multiply 128 rows of nothing, which
+// bounded 37 tokens x 65,536 at hidden 2048 by the tensor pipe (58 us) instead of by reading the head (41 us).
+template <bool SOLO>
+struct Shape {
+  static constexpr int ROWS = SOLO ? 128 : 256;
+  static constexpr int B_BYTES = SOLO ? 2 * OPERAND_BYTES : OPERAND_BYTES;
+  static constexpr int STAGE_BYTES = OPERAND_BYTES + B_BYTES;
+  static constexpr int STAGES = RING_BYTES / STAGE_BYTES;  // 4 or 6
+};
 constexpr int EPI_WARP0 = 4;
 constexpr int STG_BYTES = 32768;  // the epilogue warps' tiles on their way out
-constexpr int OFF_STG = STAGES * STAGE_BYTES;
+constexpr int OFF_STG = RING_BYTES;
 constexpr int OFF_BAR = OFF_STG + STG_BYTES;
-constexpr int NUM_BARS = 2 * STAGES + 5;
+constexpr int NUM_BARS = 2 * 6 + 5;
 constexpr int OFF_TMEM = OFF_BAR + NUM_BARS * 8;
 constexpr int SMEM_BYTES = OFF_TMEM + 16 + 1024;
 constexpr uint32_t TMEM_COLS = 512;
@@ -96,6 +106,7 @@ struct Params {
   int planes, depth;       // kAcc: the most parts the depth may be split into, each summed in a plane of its own, and
                            // a whole piece's depth, which decides how many are used
   int first;               // kAcc: the first piece (stores)
+  bool solo;               // no more than 128 tokens
 };
 
 // Into how many parts the depth k of a product of `units` tiles is split on `pairs` CTA pairs: the number whose last
@@ -127,11 +138,11 @@ struct Units {
   __device__ int k_begin(int part) const { return static_cast<int>(static_cast<int64_t>(kblocks) * part / parts); }
 };
 
-template <int MODE>
+template <int MODE, bool SOLO>
 __device__ __forceinline__ Units units_of(const Params& p, int pairs) {
   Units w;
   const int live = p.state[kLive];
-  const int row_tiles = (live + TILE - 1) / TILE;
+  const int row_tiles = (live + Shape<SOLO>::ROWS - 1) / Shape<SOLO>::ROWS;
   if (MODE == kWeight) {
     w.mt = p.piece_tiles, w.nt = (p.hidden + TILE - 1) / TILE, w.parts = 1;
     w.kblocks = (live + BK - 1) / BK;
@@ -339,13 +350,15 @@ __device__ __forceinline__ void keep_sums(const Params& p, const RowSums& s, int
   p.part[static_cast<int64_t>(SLOTS * (p.v0 / TILE + n) + half) * p.rows_pad + row] = kept;
 }
 
-template <int MODE, bool REDO, bool DEEP>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__((Epi<MODE, DEEP>::THREADS), 1)
+template <int MODE, bool REDO, bool DEEP, bool SOLO>
+__global__ void __launch_bounds__((Epi<MODE, DEEP>::THREADS), 1)
     vocab_product(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap ta32,
                   const __grid_constant__ CUtensorMap tb, const __grid_constant__ CUtensorMap tout, const Params p) {
   constexpr bool A_MN = MODE == kWeight;
   constexpr bool B_MN = MODE == kWeight || MODE == kAcc;
   using E = Epi<MODE, DEEP>;
+  using S = Shape<SOLO>;
+  constexpr int STAGES = S::STAGES;
   if (REDO) {
     let_next_start();
     wait_for_last();
@@ -355,8 +368,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__((Epi<MODE, DEEP>::TH
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t sbase = smem_u32(smem);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t rank = cluster_rank();
-  const int pair_id = static_cast<int>(cluster_id_x()), pairs = static_cast<int>(num_clusters_x());
+  const uint32_t rank = SOLO ? 0 : cluster_rank();
+  const int pair_id = SOLO ? static_cast<int>(blockIdx.x) : static_cast<int>(cluster_id_x());
+  const int pairs = SOLO ? static_cast<int>(gridDim.x) : static_cast<int>(num_clusters_x());
+  auto sync_unit = [&]() {  // the CTAs that share a unit
+    if (SOLO) __syncthreads();
+    else cluster_sync();
+  };
 
   const uint32_t bar0 = sbase + OFF_BAR;
   auto bar_full = [&](int s) { return bar0 + 8u * s; };
@@ -373,24 +391,29 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__((Epi<MODE, DEEP>::TH
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(bar_tfull(b), 1);
-      mbar_init(bar_tempty(b), 16);  // eight epilogue warps of each CTA
+      mbar_init(bar_tempty(b), SOLO ? 8 : 16);  // eight epilogue warps of each CTA
     }
     mbar_init(bar_drain, 1);
     fence_barrier_init();
   }
   if (warp == 1) {
-    tmem_alloc_pair(smem_u32(tmem_slot), TMEM_COLS);
-    tmem_relinquish_pair();
+    if (SOLO) {
+      tmem_alloc(smem_u32(tmem_slot), TMEM_COLS);
+      tmem_relinquish();
+    } else {
+      tmem_alloc_pair(smem_u32(tmem_slot), TMEM_COLS);
+      tmem_relinquish_pair();
+    }
   }
   tc_fence_before();
-  cluster_sync();
+  sync_unit();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   if (!REDO) {
     let_next_start();
     wait_for_last();
   }
-  const Units w = units_of<MODE>(p, pairs);
+  const Units w = units_of<MODE, SOLO>(p, pairs);
   const int live = p.state[kLive];
   if (MODE == kAcc && blockIdx.x == 0 && threadIdx.x == 0) p.state[kParts] = w.parts;
 
@@ -411,34 +434,43 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__((Epi<MODE, DEEP>::TH
         int m, n, part;
         w.decode(u, m, n, part);
         if (REDO && p.flags[m] == 0) continue;
-        const int a0 = m * TILE + 128 * static_cast<int>(rank), b0 = n * TILE + 128 * static_cast<int>(rank);
+        const int a0 = m * S::ROWS + 128 * static_cast<int>(rank), b0 = n * TILE + 128 * static_cast<int>(rank);
         const int k1 = w.k_begin(part + 1);
         // of a row tile that is not full only the runs of 32 rows that hold live ones are loaded; what stands in the
         // others' places meets nothing but its own rows of the accumulator
-        const int have = A_MN ? TILE : live - m * TILE;
-        const int runs0 = min(4, max(0, (have + 31) / 32)), runs1 = min(4, max(0, (have - 128 + 31) / 32));
+        const int have = A_MN ? TILE : live - m * S::ROWS;
+        const int runs0 = min(4, max(0, (have + 31) / 32)), runs1 = SOLO ? 0 : min(4, max(0, (have - 128 + 31) / 32));
         const int runs = rank == 0 ? runs0 : runs1;
         const uint32_t bytes = 2 * OPERAND_BYTES + static_cast<uint32_t>(runs0 + runs1) * (OPERAND_BYTES / 4);
         for (int kb = w.k_begin(part); kb < k1; ++kb) {
           if (!mbar_wait(bar_empty(stage), phase ^ 1)) { ok = false; break; }
-          const uint32_t fb = map_to_rank(bar_full(stage), 0);
-          const uint32_t a_dst = sbase + stage * STAGE_BYTES, b_dst = a_dst + OPERAND_BYTES;
+          const uint32_t fb = SOLO ? bar_full(stage) : map_to_rank(bar_full(stage), 0);
+          const uint32_t a_dst = sbase + stage * S::STAGE_BYTES, b_dst = a_dst + OPERAND_BYTES;
           const int k0 = kb * BK;
+          auto load = [&](uint32_t dst, const CUtensorMap* map, int x, int y) {
+            if (SOLO) tma_load_2d(dst, map, fb, x, y);
+            else tma_load_2d_pair(dst, map, fb, x, y);
+          };
           if (rank == 0) mbar_arrive_expect_tx(bar_full(stage), bytes);
           if (A_MN) {
-            tma_load_2d_pair(a_dst, &ta, fb, a0, k0);
-            tma_load_2d_pair(a_dst + 8192, &ta, fb, a0 + 64, k0);
+            load(a_dst, &ta, a0, k0);
+            load(a_dst + 8192, &ta, a0 + 64, k0);
           } else if (runs == 4) {
-            tma_load_2d_pair(a_dst, &ta, fb, k0, a0);
+            load(a_dst, &ta, k0, a0);
           } else {
-            for (int i = 0; i < runs; ++i) tma_load_2d_pair(a_dst + i * (OPERAND_BYTES / 4), &ta32, fb, k0, a0 + 32 * i);
+            for (int i = 0; i < runs; ++i) load(a_dst + i * (OPERAND_BYTES / 4), &ta32, k0, a0 + 32 * i);
           }
-          if (B_MN) {
-            const int kr = MODE == kAcc ? p.v0 + k0 : k0;
-            tma_load_2d_pair(b_dst, &tb, fb, b0, kr);
-            tma_load_2d_pair(b_dst + 8192, &tb, fb, b0 + 64, kr);
-          } else {
-            tma_load_2d_pair(b_dst, &tb, fb, k0, p.v0 + b0);
+#pragma unroll
+          for (int i = 0; i < S::B_BYTES / OPERAND_BYTES; ++i) {
+            const uint32_t dst = b_dst + i * OPERAND_BYTES;
+            const int at = b0 + 128 * i;
+            if (B_MN) {
+              const int kr = MODE == kAcc ? p.v0 + k0 : k0;
+              load(dst, &tb, at, kr);
+              load(dst + 8192, &tb, at + 64, kr);
+            } else {
+              load(dst, &tb, k0, p.v0 + at);
+            }
           }
           issued[stage] = true;
           last_parity[stage] = phase;
@@ -449,7 +481,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__((Epi<MODE, DEEP>::TH
         for (int s = 0; s < STAGES; ++s)
           if (issued[s]) mbar_wait_drain(bar_full(s), last_parity[s]);
     } else if (warp == 1 && lane == 0 && rank == 0) {  // -------------------------------------------------------- MMA issuer (the leader)
-      constexpr uint32_t IDESC = idesc_bf16(256, 256, A_MN, B_MN);
+      constexpr uint32_t IDESC = idesc_bf16(S::ROWS, TILE, A_MN, B_MN);
+      auto mma = [&](uint32_t d, uint64_t a, uint64_t b, uint32_t add) {
+        if (SOLO) mma_bf16(d, a, b, IDESC, add);
+        else mma_bf16_pair(d, a, b, IDESC, add);
+      };
+      auto commit = [&](uint32_t bar) {
+        if (SOLO) mma_commit(bar);
+        else mma_commit_pair(bar);
+      };
       const uint64_t a_desc0 = A_MN ? smem_desc(sbase, 8192, 1024, 2) : smem_desc(sbase, 16, 1024, 2);
       const uint64_t b_desc0 = B_MN ? smem_desc(sbase + OPERAND_BYTES, 8192, 1024, 2)
                                     : smem_desc(sbase + OPERAND_BYTES, 16, 1024, 2);
@@ -465,7 +505,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__((Epi<MODE, DEEP>::TH
         const int passes = DEEP ? (w.kblocks + DEEP_BLOCKS - 1) / DEEP_BLOCKS : 1;
         for (int pass = 0; pass < passes && ok; ++pass) {
           const int ab = it & 1;
-          if (!mbar_wait_cluster(bar_tempty(ab), ((it >> 1) & 1) ^ 1)) { ok = false; break; }
+          const uint32_t freed = ((it >> 1) & 1) ^ 1;
+          if (!(SOLO ? mbar_wait(bar_tempty(ab), freed) : mbar_wait_cluster(bar_tempty(ab), freed))) { ok = false; break; }
           tc_fence_after();
           const uint32_t d = tmem_base + ab * TILE;
           const int k0 = DEEP ? w.kblocks * pass / passes : w.k_begin(part);
@@ -473,21 +514,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__((Epi<MODE, DEEP>::TH
           for (int kb = k0; kb < k1; ++kb) {
             if (!mbar_wait(bar_full(stage), phase)) { ok = false; break; }
             tc_fence_after();
-            const uint64_t a_st = a_desc0 + static_cast<uint32_t>(stage) * (STAGE_BYTES / 16);
-            const uint64_t b_st = b_desc0 + static_cast<uint32_t>(stage) * (STAGE_BYTES / 16);
-            mma_bf16_pair(d, a_st, b_st, IDESC, kb != k0);
+            const uint64_t a_st = a_desc0 + static_cast<uint32_t>(stage) * (S::STAGE_BYTES / 16);
+            const uint64_t b_st = b_desc0 + static_cast<uint32_t>(stage) * (S::STAGE_BYTES / 16);
+            mma(d, a_st, b_st, kb != k0);
 #pragma unroll
-            for (int kk = 1; kk < BK / 16; ++kk) mma_bf16_pair(d, a_st + A_KK * kk, b_st + B_KK * kk, IDESC, 1);
-            mma_commit_pair(bar_empty(stage));
+            for (int kk = 1; kk < BK / 16; ++kk) mma(d, a_st + A_KK * kk, b_st + B_KK * kk, 1);
+            commit(bar_empty(stage));
             if (++stage == STAGES) stage = 0, phase ^= 1;
           }
           if (!ok) break;
-          mma_commit_pair(bar_tfull(ab));
+          commit(bar_tfull(ab));
           ++it;
         }
       }
       if (!ok) {
-        mma_commit_pair(bar_drain);
+        commit(bar_drain);
         mbar_wait_drain(bar_drain, 0);
       }
     }
@@ -498,7 +539,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__((Epi<MODE, DEEP>::TH
     auto release = [&](uint32_t bar) {  // the warp is done with an accumulator: one arrival for its 32 lanes
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive_remote(bar, 0);
+      if (lane == 0) {
+        if (SOLO) mbar_arrive(bar);
+        else mbar_arrive_remote(bar, 0);
+      }
     };
     // the next unit, and what is known of this thread's row in it, are looked up a unit ahead
     const int row_in_tile = 128 * static_cast<int>(rank) + 32 * q;
@@ -508,14 +552,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__((Epi<MODE, DEEP>::TH
     RowIn next;
     if (first < w.total) {
       w.decode(first, m, n, part);
-      next = row_in<MODE>(p, m * TILE + row_in_tile + lane, live);
+      next = row_in<MODE>(p, m * S::ROWS + row_in_tile + lane, live);
     }
     for (int u = first; u < w.total; u += step) {
-      const int row0 = m * TILE + row_in_tile, c_first = n * TILE + half * 128, tile_n = n, tile_m = m, my_part = part;
+      const int row0 = m * S::ROWS + row_in_tile, c_first = n * TILE + half * 128, tile_n = n, tile_m = m, my_part = part;
       const RowIn in = next;
       if (u + step < w.total) {
         w.decode(u + step, m, n, part);
-        next = row_in<MODE>(p, m * TILE + row_in_tile + lane, live);
+        next = row_in<MODE>(p, m * S::ROWS + row_in_tile + lane, live);
       }
       if (REDO) {
         if (p.flags[tile_m] == 0) continue;
@@ -585,10 +629,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__((Epi<MODE, DEEP>::TH
   }
 
   tc_fence_before();
-  cluster_sync();
+  sync_unit();
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc_pair(tmem_base, TMEM_COLS);
+    if (SOLO) tmem_dealloc(tmem_base, TMEM_COLS);
+    else tmem_dealloc_pair(tmem_base, TMEM_COLS);
   }
 }
 
@@ -891,22 +936,36 @@ __global__ void __launch_bounds__(256) vocab_finish(const float* __restrict__ ac
 
 // `after`: as a programmatic dependent of the launch before it on the stream (one of this call's, which all wait).
 template <typename... P>
-static int launch_chained(bool after, void (*kern)(P...), unsigned grid, unsigned threads, size_t smem, cudaStream_t s,
-                          P... args) {
-  cudaLaunchAttribute attr = {};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
+static int launch_in(unsigned cluster, bool after, void (*kern)(P...), unsigned grid, unsigned threads, size_t smem,
+                     cudaStream_t s, P... args) {
+  cudaLaunchAttribute attr[2] = {};
+  int n = 0;
+  if (after) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (cluster > 1) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = cluster, attr[n].val.clusterDim.y = 1, attr[n].val.clusterDim.z = 1;
+    ++n;
+  }
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3(grid), config.blockDim = dim3(threads), config.dynamicSmemBytes = smem, config.stream = s;
-  config.attrs = &attr, config.numAttrs = after ? 1 : 0;
+  config.attrs = attr, config.numAttrs = n;
   if (cudaLaunchKernelEx(&config, kern, args...) != cudaSuccess) return cudaGetLastError(), MEEP2B_ERR_LAUNCH;
   return MEEP2B_OK;
 }
 
-template <int MODE, bool REDO, bool DEEP>
+template <typename... P>
+static int launch_chained(bool after, void (*kern)(P...), unsigned grid, unsigned threads, size_t smem, cudaStream_t s,
+                          P... args) {
+  return launch_in<P...>(1, after, kern, grid, threads, smem, s, args...);
+}
+
+template <int MODE, bool REDO, bool DEEP, bool SOLO>
 static int launch_product(const CUtensorMap& a, const CUtensorMap& a32, const CUtensorMap& b, const CUtensorMap& out,
                           const Params& p, int pairs, cudaStream_t s, bool after) {
-  auto kern = vocab_product<MODE, REDO, DEEP>;
+  auto kern = vocab_product<MODE, REDO, DEEP, SOLO>;
   static uint64_t configured = 0;  // per device: a function's attributes are set on the current one
   int device = 0;
   if (cudaGetDevice(&device) != cudaSuccess) return cudaGetLastError(), MEEP2B_ERR_LAUNCH;
@@ -920,16 +979,26 @@ static int launch_product(const CUtensorMap& a, const CUtensorMap& a32, const CU
     }
     if (device < 64) configured |= uint64_t(1) << device;
   }
-  return launch_chained(after, kern, 2u * pairs, Epi<MODE, DEEP>::THREADS, SMEM_BYTES, s, a, a32, b, out, p);
+  return launch_in(SOLO ? 1 : 2, after, kern, 2u * pairs, Epi<MODE, DEEP>::THREADS, SMEM_BYTES, s, a, a32, b, out, p);
 }
 
 template <int MODE, bool REDO>
 static int launch(const CUtensorMap& a, const CUtensorMap& a32, const CUtensorMap& b, const CUtensorMap& out,
                   const Params& p, int pairs, cudaStream_t s, bool after = true) {
-  if constexpr (MODE != kAcc && MODE != kWeight) {
-    if (p.hidden > DEEP_BLOCKS * BK) return launch_product<MODE, REDO, true>(a, a32, b, out, p, pairs, s, after);
+  constexpr bool LOGITS = MODE != kAcc && MODE != kWeight;
+  const bool deep = p.hidden > DEEP_BLOCKS * BK;
+  if constexpr (MODE != kWeight) {
+    if (p.solo) {
+      if constexpr (LOGITS) {
+        if (deep) return launch_product<MODE, REDO, true, true>(a, a32, b, out, p, pairs, s, after);
+      }
+      return launch_product<MODE, REDO, false, true>(a, a32, b, out, p, pairs, s, after);
+    }
   }
-  return launch_product<MODE, REDO, false>(a, a32, b, out, p, pairs, s, after);
+  if constexpr (LOGITS) {
+    if (deep) return launch_product<MODE, REDO, true, false>(a, a32, b, out, p, pairs, s, after);
+  }
+  return launch_product<MODE, REDO, false, false>(a, a32, b, out, p, pairs, s, after);
 }
 
 static int map_bf16(CUtensorMap* map, const void* base, int64_t inner, int64_t rows, int64_t ld, uint32_t box_inner,
@@ -982,6 +1051,7 @@ vocab::Params params_of(const meep2b_linear_ce* a) {
   p.part = a->part, p.rows_pad = a->rows_pad, p.upstream = a->upstream;
   p.per_token = a->reduction == MEEP2B_REDUCE_NONE, p.mean = a->reduction == MEEP2B_REDUCE_MEAN;
   p.vocab = static_cast<int>(a->vocab), p.hidden = static_cast<int>(a->hidden_size), p.planes = a->planes;
+  p.solo = a->tokens <= 128;
   p.depth = static_cast<int>(a->piece_cols > 0 && a->piece_cols < a->vocab ? a->piece_cols : a->vocab);
   return p;
 }
