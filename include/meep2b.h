@@ -377,7 +377,7 @@ enum meep2b_reduction { MEEP2B_REDUCE_NONE = 0, MEEP2B_REDUCE_MEAN = 1, MEEP2B_R
  * (multiples of 8, as is hidden_size; 16-byte aligned); targets (tokens) int64, `ignore_index` where there is none:
  * such a token's loss and gradient are zero and nothing of its row is read. A target outside the vocabulary makes its
  * token's loss and gradient NaN. The mean is over the tokens with a target (zero where there are none). At most 2^24
- * tokens and 2^24 vocabulary rows. Sizes of the buffers come from meep2b_linear_ce_plan. */
+ * tokens and 2^24 vocabulary rows, and 2^44 of both multiplied. Sizes of the buffers come from meep2b_linear_ce_plan. */
 typedef struct meep2b_linear_ce {
   const void* hidden;
   int64_t tokens;

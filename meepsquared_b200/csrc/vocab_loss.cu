@@ -1030,6 +1030,7 @@ int pairs_of_device(int* pairs) {
 int check_linear_ce(const meep2b_linear_ce* a, bool forward) {
   if (a == nullptr || a->tokens < 0 || a->hidden_size < 1 || a->vocab < 1) return MEEP2B_ERR_SHAPE;
   if (a->tokens > (1 << 24) || a->vocab > (1 << 24) || a->hidden_size > (1 << 20)) return MEEP2B_ERR_SHAPE;
+  if ((a->tokens / 256 + 1) * (a->vocab / 256 + 1) > (1 << 28)) return MEEP2B_ERR_SHAPE;  // units are counted in 32 bits
   if (a->hidden_size % 8 || a->ld_weight % 8 || a->ld_weight < a->hidden_size || !aligned16(a->weight))
     return MEEP2B_ERR_ALIGN;
   if (forward && (a->ld_hidden % 8 || !aligned16(a->hidden))) return MEEP2B_ERR_ALIGN;
