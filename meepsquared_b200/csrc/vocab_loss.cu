@@ -17,13 +17,17 @@
 // below), which also keeps what stands in ignored rows, infinities and NaN included, out of every sum.
 //
 // The products are one persistent tcgen05 kernel on CTA pairs (M = 256, N = 256, K = 64 a stage, both operands by
-// TMA, two accumulators in tensor memory), or on single CTAs for few tokens, with a mode for each epilogue:
+// TMA, two accumulators in tensor memory), or on single CTAs for few rows, with a mode for each epilogue:
 //   kStats    the row sums of a 256-column tile (its two halves), nothing else
 //   kProbs    the same, and q as bf16 into the vocabulary piece's buffer
 //   kReprobs  q alone, for the row tiles to be computed again
 //   kGrad     g (q / Z - [v = y]) as bf16 into the piece's buffer (the head's gradient, and dh beside it)
 //   kAcc      dh's product: piece x W, float32, stored by the first piece and added (TMA reduction) by the others
 //   kWeight   dW's product: piece^T x h, bf16
+//
+// Bound by the tensor pipe where hidden and rows are large (82-88% active alone; 16,384 tokens x 131,072 at hidden 2048, loss
+// and dh: 13.4-13.9 ms, 1.27-1.32 PFLOP/s at the power cap), by the epilogue's exponentials below hidden 512 or so (8,192 tokens
+// x 50,000 at hidden 64: 174 us), and by reading the head for few rows (37 tokens x 131,072: 104 us for 537 MB).
 //
 // The tensor cores cut every step's sum off toward zero. Over the 256 steps of a logit of 4,096 products that made the
 // mean loss 1.1e-6 of itself too small; so beyond 2,048 products a logit's sum is taken from tensor memory every 2,048
@@ -39,9 +43,15 @@ constexpr int BK = 64;
 constexpr int OPERAND_BYTES = 128 * BK * 2;  // 128 rows or columns of an operand, one stage
 constexpr int RING_BYTES = 192 * 1024;
 
-// A unit is 256 rows on a CTA pair, each CTA with its 128 rows and half of the 256 columns; or (SOLO), where a call has
-// no more than 128 tokens, 128 rows on one CTA with all 256 columns: a pair would multiply 128 rows of nothing, which
-// bounded 37 tokens x 65,536 at hidden 2048 by the tensor pipe (58 us) instead of by reading the head (41 us).
+// A unit is 256 rows on a CTA pair, each CTA with its 128 rows and half of the 256 columns; or (SOLO) 128 rows on one CTA
+// with all 256 columns, which loads half as much again for each product. Single CTAs are taken where a pair's last 128
+// rows would be empty and are a good part of all (few_rows: an odd number of 128-row tiles, up to five). Loss alone at
+// hidden 2048, vocabulary 131,072, pairs against single CTAs: 37 tokens 117 and 104 us, 200 tokens 127 and 140, 300 tokens
+// 217 and 180, 512 tokens 204 and 219.
+inline bool few_rows(int64_t tokens) {
+  const int64_t tiles = (tokens + 127) / 128;
+  return tiles % 2 == 1 && tiles <= 5;
+}
 template <bool SOLO>
 struct Shape {
   static constexpr int ROWS = SOLO ? 128 : 256;
@@ -106,7 +116,7 @@ struct Params {
   int planes, depth;       // kAcc: the most parts the depth may be split into, each summed in a plane of its own, and
                            // a whole piece's depth, which decides how many are used
   int first;               // kAcc: the first piece (stores)
-  bool solo;               // no more than 128 tokens
+  bool solo;               // see Shape
 };
 
 // Into how many parts the depth k of a product of `units` tiles is split on `pairs` CTA pairs: the number whose last
@@ -433,7 +443,7 @@ __global__ void __launch_bounds__((Epi<MODE, DEEP>::THREADS), 1)
       for (int u = pair_id; u < w.total && ok; u += pairs) {
         int m, n, part;
         w.decode(u, m, n, part);
-        if (REDO && p.flags[m] == 0) continue;
+        if (REDO && p.flags[m * S::ROWS / TILE] == 0) continue;
         const int a0 = m * S::ROWS + 128 * static_cast<int>(rank), b0 = n * TILE + 128 * static_cast<int>(rank);
         const int k1 = w.k_begin(part + 1);
         // of a row tile that is not full only the runs of 32 rows that hold live ones are loaded; what stands in the
@@ -501,7 +511,7 @@ __global__ void __launch_bounds__((Epi<MODE, DEEP>::THREADS), 1)
       for (int u = pair_id; u < w.total && ok; u += pairs) {
         int m, n, part;
         w.decode(u, m, n, part);
-        if (REDO && p.flags[m] == 0) continue;
+        if (REDO && p.flags[m * S::ROWS / TILE] == 0) continue;
         const int passes = DEEP ? (w.kblocks + DEEP_BLOCKS - 1) / DEEP_BLOCKS : 1;
         for (int pass = 0; pass < passes && ok; ++pass) {
           const int ab = it & 1;
@@ -562,7 +572,7 @@ __global__ void __launch_bounds__((Epi<MODE, DEEP>::THREADS), 1)
         next = row_in<MODE>(p, m * S::ROWS + row_in_tile + lane, live);
       }
       if (REDO) {
-        if (p.flags[tile_m] == 0) continue;
+        if (p.flags[tile_m * S::ROWS / TILE] == 0) continue;
         if (E::GROUPS == 2 && (it & 1) != group) {
           ++it;
           continue;
@@ -1052,7 +1062,7 @@ vocab::Params params_of(const meep2b_linear_ce* a) {
   p.part = a->part, p.rows_pad = a->rows_pad, p.upstream = a->upstream;
   p.per_token = a->reduction == MEEP2B_REDUCE_NONE, p.mean = a->reduction == MEEP2B_REDUCE_MEAN;
   p.vocab = static_cast<int>(a->vocab), p.hidden = static_cast<int>(a->hidden_size), p.planes = a->planes;
-  p.solo = a->tokens <= 128;
+  p.solo = vocab::few_rows(a->tokens);
   p.depth = static_cast<int>(a->piece_cols > 0 && a->piece_cols < a->vocab ? a->piece_cols : a->vocab);
   return p;
 }

@@ -97,7 +97,8 @@ def check(h, w, t, reduction, head, seed=3):
 @pytest.mark.parametrize("tokens,hidden,vocab", [(1, 8, 1), (1, 64, 7), (2, 72, 256), (37, 200, 257), (255, 64, 1000),
                                                  (257, 128, 513), (300, 512, 5003), (700, 264, 2048),
                                                  (70, 2048, 300), (70, 2056, 300), (300, 4104, 1000),
-                                                 (5, 8200, 700)])
+                                                 (5, 8200, 700), (128, 72, 600), (129, 72, 600), (384, 72, 600),
+                                                 (385, 2056, 600), (640, 72, 900)])
 def test_losses_and_gradients(tokens, hidden, vocab, head):
     h, w, t = inputs(tokens, hidden, vocab)
     check(h, w, t, "none", head)
@@ -136,17 +137,18 @@ def test_pieces_and_planes(monkeypatch, piece_cols, planes, head):
     check(h, w, t, "none", head)
 
 
+@pytest.mark.parametrize("tokens", [100, 350, 700])
 @pytest.mark.parametrize("hidden", [64, 2104])
 @pytest.mark.parametrize("pieces", [False, True], ids=["whole", "pieces"])
-def test_targets_far_below_the_largest_logit(monkeypatch, pieces, hidden):
+def test_targets_far_below_the_largest_logit(monkeypatch, pieces, hidden, tokens):
     """Logits hundreds above the target's: beyond the window of the target's own reference, in some rows of some
     tiles (the others keep theirs), and far below it."""
     if pieces:
         monkeypatch.setattr(_loss, "PLAN", (512, 2))
-    h, w, t = inputs(700, hidden, 1500)
-    far = torch.arange(700, device=DEV) % 97 == 5
+    h, w, t = inputs(tokens, hidden, 1500)
+    far = torch.arange(tokens, device=DEV) % 97 == 5
     h[far] *= 200.0   # logits of +-600 or so
-    h[600:] *= 30.0   # around the window's edge
+    h[tokens * 6 // 7:] *= 30.0   # around the window's edge
     check(h, w, t, "none", False)
     check(h, w, t, "none", True)
 
