@@ -216,3 +216,39 @@ def test_refusals():
         mb.balance_loss(torch.zeros((4, 1025), device=DEV), 2)
     with pytest.raises(ValueError, match="128"):
         mb.balance_loss([x] * 129, 2)
+
+
+def test_offsets_past_32_bits():
+    """More than 2^31 logits: the counts of all tokens against the choice in pieces, and the last rows' gradient."""
+    tokens, experts = 17_000_003, 128
+    gen = torch.Generator(device=DEV).manual_seed(1)
+    x = torch.empty((tokens, experts), dtype=torch.bfloat16, device=DEV).normal_(generator=gen).requires_grad_()
+    loss, counts = mb.balance_loss(x, 4)
+    grad, = torch.autograd.grad(loss, x)
+    assert int(counts.sum()) == 4 * tokens
+    want = torch.zeros(experts, dtype=torch.int64, device=DEV)
+    mass = torch.zeros(experts, dtype=torch.float64, device=DEV)
+    for rows in x.detach().split(1 << 20):
+        key = rows.float().view(torch.int32).long()
+        key = torch.where(key < 0, -(key & 0x7FFFFFFF), key) * 1024 - torch.arange(experts, device=DEV)
+        want += torch.bincount(key.topk(4, dim=1)[1].reshape(-1), minlength=experts)
+        mass += torch.softmax(rows.float(), 1).sum(0, dtype=torch.float64)
+    assert torch.equal(counts, want)
+    f = want.double() / tokens
+    assert abs(float(loss.detach()) - float(experts * (f * mass).sum() / tokens)) <= 1e-5 * float(loss.detach())
+    p = torch.softmax(x.detach()[-100:].double(), 1)
+    f = f - f.mean()
+    dx = experts / tokens * p * (f - (p * f).sum(1, keepdim=True))
+    tol = 1e-5 * experts / tokens * p * (f.abs() + (p * f.abs()).sum(1, keepdim=True)) + 1.01 * 2.0 ** -8 * dx.abs()
+    assert bool(((grad[-100:].double() - dx).abs() <= tol + 1e-38).all())
+
+
+def test_recomputed_under_a_checkpoint():
+    from torch.utils.checkpoint import checkpoint
+
+    xs = make(2, 50, 16, torch.float32)
+    a = [x.detach().requires_grad_() for x in xs]
+    mb.balance_loss(a, 2)[0].backward()
+    b = [x.detach().requires_grad_() for x in xs]
+    checkpoint(lambda *y: mb.balance_loss(y, 2)[0], *b, use_reentrant=False).backward()
+    assert all(torch.equal(x.grad, y.grad) for x, y in zip(a, b))

@@ -274,3 +274,35 @@ def test_refusals():
         mb.qk_norm_rope(q, k, wq, wk, cos, sin, positions=torch.zeros(4, dtype=torch.int64, device=DEV))
     with pytest.raises(TypeError, match="positions"):
         mb.qk_norm_rope(q, k, wq, wk, cos, sin, positions=torch.zeros((1, 4), device=DEV))
+
+
+def test_offsets_past_32_bits():
+    """More than 2^31 values of queries, in a slice of a fused projection: the last tokens against the formula."""
+    tokens, d = 530_001, 128
+    gen = torch.Generator(device=DEV).manual_seed(1)
+    fused = torch.empty((1, tokens, 34, d), dtype=torch.bfloat16, device=DEV).normal_(generator=gen)
+    q, k = fused[:, :, :33].requires_grad_(), fused[:, :, 33:].detach()
+    wq, wk = (1 + 0.1 * torch.randn(d, device=DEV, generator=gen)).bfloat16(), torch.ones(d, device=DEV).bfloat16()
+    cos, sin = angles(1000, 64)
+    pos = (torch.arange(tokens, device=DEV) % 1000)[None]
+    out = mb.qk_norm_rope(q, k, wq, wk, cos, sin, positions=pos)
+    dy = torch.empty_like(out[0]).normal_(generator=gen)
+    grad, = torch.autograd.grad(out[0], q, dy)
+    for at in (slice(0, 10), slice(tokens - 10, tokens)):
+        c, s = cos.double()[pos[:, at]][:, :, None], sin.double()[pos[:, at]][:, :, None]
+        y, dx, _ = formula(q.detach()[:, at], wq, c, s, 1e-6, dy[:, at])
+        near(out[0].detach()[:, at], y, "out")
+        near(grad[:, at], dx, "dx")
+
+
+def test_recomputed_under_a_checkpoint():
+    from torch.utils.checkpoint import checkpoint
+
+    parts = make(1, 40, 4, 2, 64, torch.bfloat16)
+    cos, sin = angles(40, 32)
+    a = [x.detach().requires_grad_() for x in parts[:4]]
+    want = torch.autograd.grad(mb.qk_norm_rope(*a, cos, sin), a, list(parts[4:]))
+    b = [x.detach().requires_grad_() for x in parts[:4]]
+    out = checkpoint(lambda *y: mb.qk_norm_rope(*y, cos, sin), *b, use_reentrant=False)
+    got = torch.autograd.grad(out, b, list(parts[4:]))
+    assert all(torch.equal(x, y) for x, y in zip(want, got))

@@ -315,3 +315,58 @@ def test_refusals():
         mb.linear_cross_entropy(h, w, t.float())
     with pytest.raises(ValueError, match="devices"):
         mb.linear_cross_entropy(h, w.cpu(), t)
+
+
+@pytest.mark.parametrize("long", ["rows", "head"])
+def test_offsets_past_32_bits(long):
+    """More than 2^31 values of hidden states (an odd number of tokens, two in three ignored) or of the head: losses and
+    gradients of the first and the last rows against the formula on those rows alone."""
+    tokens, vocab, hidden = (1100001, 300, 2048) if long == "rows" else (40, 1100001, 2048)
+    gen = torch.Generator(device=DEV).manual_seed(1)
+    h = torch.empty((tokens, hidden), dtype=torch.bfloat16, device=DEV).normal_(generator=gen)
+    w = torch.empty((vocab, hidden), dtype=torch.bfloat16, device=DEV).normal_(0.0, hidden ** -0.5, generator=gen)
+    t = torch.randint(0, vocab, (tokens,), device=DEV, generator=gen)
+    t[:2], t[-2:] = 0, vocab - 1
+    if long == "rows":
+        t[1000:-1000][torch.arange(tokens - 2000, device=DEV) % 3 != 0] = -100
+    up = torch.ones((tokens,), device=DEV)
+    h.requires_grad_()
+    loss = mb.linear_cross_entropy(h, w, t, reduction="none")
+    loss.backward(up)
+    ends = torch.cat([torch.arange(20, device=DEV), torch.arange(tokens - 20, tokens, device=DEV)])
+    part = h.detach()[ends].double()
+    z = torch.cat([part @ w[i:i + 65536].double().t() for i in range(0, vocab, 65536)], 1)
+    lse = torch.logsumexp(z, 1)
+    at = torch.arange(40, device=DEV)
+    d = (hidden / 16 + 16) * 2.0 ** -23 * float((part[:2].abs() @ w[:20000].double().abs().t()).max()) * 2
+    want = lse - z[at, t[ends]]
+    assert float((loss.detach()[ends].double() - want).abs().max()) <= 2 * d + 2.0 ** -20 * float(want.max())
+    p = torch.exp(z - lse[:, None])
+    p[at, t[ends]] -= 1.0
+    dh = sum(p[:, i:i + 65536] @ w[i:i + 65536].double() for i in range(0, vocab, 65536))
+    assert float((h.grad[ends].double() - dh).norm()) <= 2.0 ** -8 * float(dh.norm())
+    assert not h.grad[t == -100].any() if long == "rows" else True
+    assert torch.isfinite(loss).all() and _lib.device_error(0) == 0
+
+
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_recomputed_under_a_checkpoint(reentrant):
+    from torch.utils.checkpoint import checkpoint
+
+    h, w, t = inputs(200, 64, 500, ignored=0.2)
+    for head in (False, True):
+        a, b = h.detach().requires_grad_(), w.detach().requires_grad_(head)
+        mb.linear_cross_entropy(a, b, t).backward()
+        c, d = h.detach().requires_grad_(), w.detach().requires_grad_(head)
+        checkpoint(lambda x, y: mb.linear_cross_entropy(x, y, t), c, d, use_reentrant=reentrant).backward()
+        assert torch.equal(a.grad, c.grad) and (not head or torch.equal(b.grad, d.grad))
+
+
+def test_saved_on_the_host_in_between():
+    h, w, t = inputs(200, 64, 500, ignored=0.2)
+    a, b, c, d = (x.detach().requires_grad_() for x in (h, w, h, w))
+    mb.linear_cross_entropy(a, b, t).backward()
+    with torch.autograd.graph.save_on_cpu():
+        loss = mb.linear_cross_entropy(c, d, t)
+    loss.backward()
+    assert torch.equal(a.grad, c.grad) and torch.equal(b.grad, d.grad)
