@@ -399,11 +399,12 @@ typedef struct meep2b_linear_ce {
   int32_t* slot;           /* tokens: live row of each token, or -1 */
   int32_t* target;         /* rows_pad */
   float* row_values;       /* 5 * rows_pad */
-  void* compact;           /* (rows_pad, hidden_size) bf16: the live rows (backward: only with d_weight) */
+  void* compact;           /* (rows_pad, hidden_size) bf16: the live rows. Backward: given, the gradients are computed
+                              there (acc is then a workspace); NULL, dh's planes are the forward call's (no d_weight) */
   float* acc;              /* planes * (rows_pad, hidden_size): the hidden states' gradient before its upstream scale;
                               forward: NULL for the loss alone */
   /* workspaces of one call */
-  void* piece;             /* (rows_pad, piece_cols) bf16; needed with acc (forward) and with d_weight (backward) */
+  void* piece;             /* (rows_pad, piece_cols) bf16; needed with acc (forward) and with compact (backward) */
   float* part;             /* 2 * ceil(vocab / 256) * rows_pad (forward) */
   float* row_loss;         /* rows_pad (forward, mean and sum) */
   /* forward: tokens values (none) or one */
@@ -411,8 +412,7 @@ typedef struct meep2b_linear_ce {
   /* backward: the loss's gradient (tokens values or one), and what is asked for, contiguous */
   const float* upstream;
   void* d_hidden;          /* (tokens, hidden_size) bf16, or NULL */
-  void* d_weight;          /* (vocab, hidden_size) bf16, or NULL: the frozen head. With it the gradients are computed
-                              by the backward call (acc is then its workspace), else dh's planes by the forward call */
+  void* d_weight;          /* (vocab, hidden_size) bf16, or NULL */
 } meep2b_linear_ce;
 
 /* rows_pad, piece_cols and planes for these sizes: a piece's buffer is at most 1 GB (or 256 columns), the planes

@@ -326,19 +326,18 @@ struct LinearCrossEntropyBackward : torch::autograd::Node {
     if (hidden) out[0] = at::empty({t.numel(), size}, w.options()), a.d_hidden = data<void>(out[0]);
     Tensor scratch;
     if (trained) {  // the planes are computed here, with or without the head's gradient
-      out[1] = at::empty({w.size(0), size}, w.options());
+      if (head) out[1] = at::empty({w.size(0), size}, w.options()), a.d_weight = data<void>(out[1]);
       Parts parts;
       const int piece = parts.add(2 * plan.rows_pad * plan.piece_cols);
       const int acc = parts.add(hidden ? 4 * int64_t(plan.planes) * plan.rows_pad * size : 0);
       scratch = parts.take(w);
-      a.compact = data<void>(last_), a.d_weight = data<void>(out[1]);
+      a.compact = data<void>(last_);
       a.piece = data<uint8_t>(scratch) + parts.at[piece];
       if (hidden) a.acc = reinterpret_cast<float*>(data<uint8_t>(scratch) + parts.at[acc]);
     } else {
       a.acc = data<float>(last_);
     }
     if (hidden || head) check(meep2b_linear_ce_backward(&a, stream_of(w)), "meep2b_linear_ce_backward");
-    if (!head) out[1] = Tensor();
     return once(std::move(out), "linear_cross_entropy");
   }
 };

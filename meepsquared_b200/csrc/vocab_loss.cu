@@ -1197,21 +1197,22 @@ int meep2b_linear_ce_backward(const meep2b_linear_ce* a, void* stream) {
   MEEP2B_TRY(bind_stream_device(s));
   int pairs = 0;
   MEEP2B_TRY(pairs_of_device(&pairs));
-  const bool recompute = a->d_weight != nullptr;  // else the forward pass left dh's planes
-  if (recompute && a->piece == nullptr) return MEEP2B_ERR_SHAPE;
-  if (recompute && a->tokens == 0) {
+  const bool recompute = a->compact != nullptr;  // else the forward pass left dh's planes
+  if (recompute ? a->piece == nullptr || a->piece_cols < vocab::TILE : a->d_weight != nullptr) return MEEP2B_ERR_SHAPE;
+  if (a->d_weight != nullptr && a->tokens == 0) {
     const cudaError_t e = cudaMemsetAsync(a->d_weight, 0, static_cast<size_t>(a->vocab) * a->hidden_size * 2, s);
     return e == cudaSuccess ? MEEP2B_OK : (cudaGetLastError(), MEEP2B_ERR_LAUNCH);
   }
   bool after = false;
-  if (recompute) {
+  if (recompute && a->tokens > 0) {
     CeMaps m;
-    MEEP2B_TRY(maps_of(a, &m, a->d_hidden != nullptr, true));
+    MEEP2B_TRY(maps_of(a, &m, a->d_hidden != nullptr, a->d_weight != nullptr));
     MEEP2B_TRY(each_piece(a, params_of(a), [&](const vocab::Params& p) -> int {
       MEEP2B_TRY((vocab::launch<vocab::kGrad, false>(m.rows, m.rows32, m.head, m.piece_out, p, pairs, s, after)));
       after = true;
       if (a->d_hidden != nullptr)
         MEEP2B_TRY((vocab::launch<vocab::kAcc, false>(m.piece, m.piece32, m.head_mn, m.acc, p, pairs, s)));
+      if (a->d_weight == nullptr) return MEEP2B_OK;
       return vocab::launch<vocab::kWeight, false>(m.piece_mn, m.piece_mn, m.rows_mn, m.d_weight, p, pairs, s);
     }));
   }

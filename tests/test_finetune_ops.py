@@ -67,3 +67,32 @@ def test_attention_modules_are_found_and_patched():
     found[0].sliding_window = 128
     with pytest.raises(NotImplementedError, match="sliding window"):
         mb.model.install_attention(model)
+
+
+def test_bad_arguments_are_refused_before_anything_runs():
+    lib = _lib.load()
+    ce = _lib.LinearCE(tokens=4, hidden_size=64, ld_hidden=64, vocab=10, ld_weight=64, rows_pad=256, hidden=4096, weight=4096)
+    assert lib.meep2b_linear_ce_forward(None, None) == _lib.ERR_SHAPE
+    assert lib.meep2b_linear_ce_forward(ctypes.byref(ce), None) == _lib.ERR_SHAPE  # no loss
+    assert lib.meep2b_linear_ce_backward(ctypes.byref(ce), None) == _lib.ERR_SHAPE  # no upstream gradient
+    for field, value, status in (("hidden_size", 60, _lib.ERR_ALIGN), ("ld_weight", 56, _lib.ERR_ALIGN),
+                                 ("weight", 4098, _lib.ERR_ALIGN), ("rows_pad", 128, _lib.ERR_SHAPE),
+                                 ("vocab", 0, _lib.ERR_SHAPE), ("reduction", 3, _lib.ERR_UNSUPPORTED)):
+        bad = _lib.LinearCE.from_buffer_copy(ce)
+        setattr(bad, field, value)
+        assert lib.meep2b_linear_ce_forward(ctypes.byref(bad), None) == status, field
+    balance = _lib.Balance(logits=4096, layers=1, experts=8, tokens=4, top_k=2, dtype=_lib.BF16)
+    assert lib.meep2b_balance_loss(None, None) == _lib.ERR_SHAPE
+    for field, value, status in (("layers", 129, _lib.ERR_SHAPE), ("experts", 1025, _lib.ERR_SHAPE),
+                                 ("top_k", 9, _lib.ERR_SHAPE), ("dtype", 7, _lib.ERR_DTYPE)):
+        bad = _lib.Balance.from_buffer_copy(balance)
+        setattr(bad, field, value)
+        assert lib.meep2b_balance_loss(ctypes.byref(bad), None) == status, field
+    heads = _lib.HeadNorm(batch=1, length=4, q_heads=2, kv_heads=1, dim=64, half=32, angles=4, dtype=_lib.BF16)
+    assert lib.meep2b_head_norm_rotate(None, None) == _lib.ERR_SHAPE
+    for field, value, status in (("dim", 72, _lib.ERR_SHAPE), ("half", 36, _lib.ERR_SHAPE), ("half", 40, _lib.ERR_SHAPE),
+                                 ("angles", 3, _lib.ERR_SHAPE), ("dtype", 2, _lib.ERR_DTYPE), ("q", 4, _lib.ERR_ALIGN),
+                                 ("length", 1 << 33, _lib.ERR_SHAPE)):
+        bad = _lib.HeadNorm.from_buffer_copy(heads)
+        setattr(bad, field, value)
+        assert lib.meep2b_head_norm_rotate(ctypes.byref(bad), None) == status, field

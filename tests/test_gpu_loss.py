@@ -276,6 +276,9 @@ def test_one_gradient_without_the_other():
     alone = w.detach().requires_grad_()
     mb.linear_cross_entropy(h, alone, t).backward()
     assert torch.equal(alone.grad, both[1].grad)
+    loss = mb.linear_cross_entropy(*both, t)
+    assert torch.equal(torch.autograd.grad(loss, both[0], retain_graph=True)[0], both[0].grad)
+    assert torch.equal(torch.autograd.grad(loss, both[1])[0], both[1].grad)
 
 
 def test_captured_in_a_graph():
