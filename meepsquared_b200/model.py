@@ -139,6 +139,9 @@ def _attention_forward(self, hidden_states, position_embeddings, attention_mask=
         k, v = past_key_values.update(k, v, self.layer_idx)
     if attention_mask is None and 1 < length < k.shape[2]:
         raise NotImplementedError("several new tokens behind cached ones need an attention mask")
+    if attention_mask is not None and attention_mask.dim() != 4:
+        raise NotImplementedError("an attention mask of (batch, 1, queries, keys) is expected: load the model with "
+                                  "attn_implementation='sdpa'")
     out = torch.nn.functional.scaled_dot_product_attention(
         q, k, v, attn_mask=attention_mask, dropout_p=self.attention_dropout if self.training else 0.0,
         is_causal=attention_mask is None and length > 1, scale=self.scaling, enable_gqa=True)

@@ -75,8 +75,8 @@ def test_the_loss_matches_the_models_own(padded):
     compare(take(model), want)
 
 
-@pytest.mark.parametrize("padded", [False, True])
-def test_attention_matches_the_models_own(padded):
+@pytest.mark.parametrize("padded,own_positions", [(False, False), (True, False), (False, True)])
+def test_attention_matches_the_models_own(padded, own_positions):
     """Each attention module alone, on the inputs that the model gives it (in the whole model the two roundings send
     near-tied tokens to other experts, and the later layers then see other inputs)."""
     model = build(layers=2)
@@ -84,10 +84,14 @@ def test_attention_matches_the_models_own(padded):
     calls = []
     modules = [m for _, m in mb.model.attention_modules(model)]
     hooks = [m.register_forward_hook(lambda m, a, k, o: calls.append(k), with_kwargs=True) for m in modules]
+    positions = None
+    if own_positions:  # every sequence at positions of its own: one row of angles for every token
+        positions = torch.arange(ids.shape[1], device=DEV)[None] + torch.tensor([[0], [17], [400]], device=DEV)
     with torch.no_grad():
-        model(input_ids=ids, attention_mask=mask, use_cache=False)
+        model(input_ids=ids, attention_mask=mask, position_ids=positions, use_cache=False)
     for h in hooks:
         h.remove()
+    assert calls[0]["position_embeddings"][0].shape[0] == (3 if own_positions else 1)
 
     def run(module, kwargs, dy):
         x = kwargs["hidden_states"].detach().requires_grad_()

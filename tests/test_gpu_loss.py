@@ -373,3 +373,28 @@ def test_saved_on_the_host_in_between():
         loss = mb.linear_cross_entropy(c, d, t)
     loss.backward()
     assert torch.equal(a.grad, c.grad) and torch.equal(b.grad, d.grad)
+
+
+def test_two_streams_at_once():
+    cases = [inputs(700, 256, 4001, seed=i, ignored=0.2) for i in range(2)]
+
+    def step(case):
+        a, b = case[0].detach().requires_grad_(), case[1].detach().requires_grad_()
+        loss = mb.linear_cross_entropy(a, b, case[2])
+        loss.backward()
+        c = case[0].detach().requires_grad_()
+        mb.linear_cross_entropy(c, case[1], case[2]).backward()
+        return loss.detach(), a.grad, b.grad, c.grad
+
+    want = [step(c) for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(10):
+        for stream, case in zip(streams, cases):
+            with torch.cuda.stream(stream):
+                got.append(step(case))
+    torch.cuda.synchronize()
+    for i, result in enumerate(got):
+        assert all(torch.equal(x, y) for x, y in zip(result, want[i % 2]))
+    assert _lib.device_error(0) == 0
