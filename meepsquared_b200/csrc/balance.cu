@@ -17,12 +17,12 @@
 // and then between lanes: about 60 instructions a token at 128 experts, where top_k rounds of a maximum over all keys
 // took 140. More than 8, or float32 logits (64-bit keys), take the rounds.
 //
-// 24 layers of 16,384 x 128 bf16: forward 75 us (112 instructions a token; the integer pipe's minima and maxima bound it,
-// 1.3 TB/s), backward 43 us (4.7 TB/s); the rounds took 174 us forward.
+// 24 layers of 16,384 x 128 bf16: forward 75 us (112 instructions a token; the integer pipe's minima and maxima bound
+// it, 1.3 TB/s), backward 43 us (4.7 TB/s); the rounds took 174 us forward.
 //
 // The probabilities' sums stay in registers over a group's tokens and are joined per CTA in float32; the CTAs' sums
-// are added as 64-bit whole numbers of 2^-36, whose order does not matter, and the last CTA to finish works out the loss
-// and the gradient's coefficients.
+// are added as 64-bit whole numbers of 2^-36, whose order does not matter, and the last CTA to finish works out the
+// loss and the gradient's coefficients.
 #include "common.cuh"
 #include "host.hpp"
 

@@ -9,12 +9,13 @@
 // of 1 to 32 lanes, each with two 16-byte chunks that turn against each other (i and i + half), so that the rotation
 // needs no exchange between lanes and the norm three or four shuffles. A group takes several heads of one token in a
 // row, which keeps the token's cosines and sines and the head weight in registers. A thread's heads come through a ring
-// of its own in shared memory by 16-byte asynchronous copies, a few heads ahead: enough in flight for HBM without holding
-// registers, and with no barrier. A CTA works on queries or on keys alone. The forward pass has a group for every run of heads; the
-// backward pass with the weights' gradients has as many CTAs as the SMs hold, in proportion to the queries' and the
-// keys' heads: their sums stay in registers, are joined per CTA, and the CTAs' sums by a second kernel in a fixed order.
-// 4 x 4,096 tokens, 32 + 4 heads of 128 in bf16: forward 50 us (6.0 TB/s, 92% of the measured copy rate), backward with the
-// weights' gradients 79 us (5.7 TB/s) and 4 us; with the loads through registers, two heads ahead, 56 and 115 us.
+// of its own in shared memory by 16-byte asynchronous copies, a few heads ahead: enough in flight for HBM without
+// holding registers, and with no barrier. A CTA works on queries or on keys alone. The forward pass has a group for
+// every run of heads; the backward pass with the weights' gradients has as many CTAs as the SMs hold, in proportion
+// to the queries' and the keys' heads: their sums stay in registers, are joined per CTA, and the CTAs' sums by a
+// second kernel in a fixed order. 4 x 4,096 tokens, 32 + 4 heads of 128 in bf16: forward 50 us (6.0 TB/s, 92% of the
+// measured copy rate), backward with the weights' gradients 79 us (5.7 TB/s) and 4 us; with the loads through
+// registers, two heads ahead, 56 and 115 us.
 #include "common.cuh"
 #include "host.hpp"
 

@@ -1,7 +1,7 @@
 // The fine-tuning operators as autograd nodes: what the Python layer calls after it has checked the arguments. A node's
 // backward runs in C++ on the engine's thread, without the interpreter: for the smaller calls the host's time is the
-// operator's time (a training call of a few microseconds on the GPU took 105 to 145 us as Python Functions over ctypes).
-// The kernels are libmeep2b's, through its C ABI; buffers come from torch's allocator on the current stream.
+// operator's time (a training call of a few microseconds on the GPU took 105 to 145 us as Python Functions over
+// ctypes). The kernels are libmeep2b's, through its C ABI; buffers come from torch's allocator on the current stream.
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>

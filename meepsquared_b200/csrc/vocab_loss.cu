@@ -25,9 +25,10 @@
 //   kAcc      dh's product: piece x W, float32, stored by the first piece and added (TMA reduction) by the others
 //   kWeight   dW's product: piece^T x h, bf16
 //
-// Bound by the tensor pipe where hidden and rows are large (82-88% active alone; 16,384 tokens x 131,072 at hidden 2048, loss
-// and dh: 13.4-13.9 ms, 1.27-1.32 PFLOP/s at the power cap), by the epilogue's exponentials below hidden 512 or so (8,192 tokens
-// x 50,000 at hidden 64: 174 us), and by reading the head for few rows (37 tokens x 131,072: 104 us for 537 MB).
+// Bound by the tensor pipe where hidden and rows are large (82-88% active alone; 16,384 tokens x 131,072 at hidden
+// 2048, loss and dh: 13.2-14.2 ms, 1.23-1.34 PFLOP/s at the power cap), by the epilogue's exponentials below hidden
+// 512 or so (8,192 tokens x 50,000 at hidden 64: 174 us), and by reading the head for few rows (37 tokens x 131,072:
+// 104 us for 537 MB).
 //
 // The tensor cores cut every step's sum off toward zero. Over the 256 steps of a logit of 4,096 products that made the
 // mean loss 1.1e-6 of itself too small; so beyond 2,048 products a logit's sum is taken from tensor memory every 2,048
@@ -43,11 +44,11 @@ constexpr int BK = 64;
 constexpr int OPERAND_BYTES = 128 * BK * 2;  // 128 rows or columns of an operand, one stage
 constexpr int RING_BYTES = 192 * 1024;
 
-// A unit is 256 rows on a CTA pair, each CTA with its 128 rows and half of the 256 columns; or (SOLO) 128 rows on one CTA
-// with all 256 columns, which loads half as much again for each product. Single CTAs are taken where a pair's last 128
-// rows would be empty and are a good part of all (few_rows: an odd number of 128-row tiles, up to five). Loss alone at
-// hidden 2048, vocabulary 131,072, pairs against single CTAs: 37 tokens 117 and 104 us, 200 tokens 127 and 140, 300 tokens
-// 217 and 180, 512 tokens 204 and 219.
+// A unit is 256 rows on a CTA pair, each CTA with its 128 rows and half of the 256 columns; or (SOLO) 128 rows on one
+// CTA with all 256 columns, which loads half as much again for each product. Single CTAs are taken where a pair's
+// last 128 rows would be empty and are a good part of all (few_rows: an odd number of 128-row tiles, up to five).
+// Loss alone at hidden 2048, vocabulary 131,072, pairs against single CTAs: 37 tokens 117 and 104 us, 200 tokens 127
+// and 140, 300 tokens 217 and 180, 512 tokens 204 and 219.
 inline bool few_rows(int64_t tokens) {
   const int64_t tiles = (tokens + 127) / 128;
   return tiles % 2 == 1 && tiles <= 5;
@@ -77,11 +78,11 @@ constexpr float kWindow = 7.9228162514264338e28f;  // 2^96
 
 enum Mode { kStats, kProbs, kReprobs, kGrad, kAcc, kWeight };
 
-// Epilogue warps, in groups of 8 (four quarters of the rows, which a warp may read of tensor memory, by two halves of the
-// columns). Over the logits every element costs an exponential, and one group, each of whose warps waits for the unit,
-// loads, computes and stores in turn, left the exponentials' unit idle more than half of the time: two groups take every
-// other unit each (5,200 cycles a unit with one, the exponentials alone are 2,048, the product's time at hidden 256).
-// The other modes have time enough with one, and DEEP needs its registers.
+// Epilogue warps, in groups of 8 (four quarters of the rows, which a warp may read of tensor memory, by two halves of
+// the columns). Over the logits every element costs an exponential, and one group, each of whose warps waits for the
+// unit, loads, computes and stores in turn, left the exponentials' unit idle more than half of the time: two groups
+// take every other unit each (5,200 cycles a unit with one, the exponentials alone are 2,048, the product's time at
+// hidden 256). The other modes have time enough with one, and DEEP needs its registers.
 template <int MODE, bool DEEP>
 struct Epi {
   static constexpr int GROUPS = MODE == kAcc || MODE == kWeight || DEEP ? 1 : 2;
@@ -431,7 +432,7 @@ __global__ void __launch_bounds__((Epi<MODE, DEEP>::THREADS), 1)
   // kernel is launched with (checked there)
   if (warp < EPI_WARP0) {
     if (DEEP) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-    if (warp == 0 && lane == 0) {  // ---------------------------------------------------------------------- TMA producer (each CTA)
+    if (warp == 0 && lane == 0) {  // ------------------------------------------------------- TMA producer (each CTA)
       tma_prefetch_desc(&ta);
       tma_prefetch_desc(&tb);
       int stage = 0;
@@ -490,7 +491,7 @@ __global__ void __launch_bounds__((Epi<MODE, DEEP>::THREADS), 1)
       if (!ok && rank == 0)
         for (int s = 0; s < STAGES; ++s)
           if (issued[s]) mbar_wait_drain(bar_full(s), last_parity[s]);
-    } else if (warp == 1 && lane == 0 && rank == 0) {  // -------------------------------------------------------- MMA issuer (the leader)
+    } else if (warp == 1 && lane == 0 && rank == 0) {  // ------------------------------------ MMA issuer (the leader)
       constexpr uint32_t IDESC = idesc_bf16(S::ROWS, TILE, A_MN, B_MN);
       auto mma = [&](uint32_t d, uint64_t a, uint64_t b, uint32_t add) {
         if (SOLO) mma_bf16(d, a, b, IDESC, add);
@@ -649,8 +650,8 @@ __global__ void __launch_bounds__((Epi<MODE, DEEP>::THREADS), 1)
 
 // ---------------------------------------------------------------------------------------------------- rows
 
-// How many of a CTA's threads' earlier threads' tokens have a target, and the CTA's total (in *total): each thread gives
-// its own number. words: one int a warp.
+// How many of a CTA's threads' earlier threads' tokens have a target, and the CTA's total (in *total): each thread
+// gives its own number. words: one int a warp.
 template <int WARPS>
 __device__ __forceinline__ int scan_before(int mine, int* words, int* total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
