@@ -180,17 +180,18 @@ __device__ __forceinline__ float group_sum(float v) {
   return v;
 }
 
-// v: 2^((x - max) log2 e) of the lane's experts; returns 1 over the group's sum of them (float32).
+// v: 2^((x - max) log2 e) of the lane's experts; returns 1 over the group's sum of them (float32). The difference is
+// taken first: x log2 e - max log2 e in one fused step overflows where a row's largest logit is the type's lowest value
+// (a row whose mask leaves nothing), and is off by more than the exponent's range from 1e10 on.
 template <int G, int PER, typename R>
 __device__ __forceinline__ float softmax(const R& row, float (&v)[PER]) {
   float top = row.largest();
 #pragma unroll
   for (int off = G / 2; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-  const float shift = -top * kLog2e;
   float sum = 0.f;
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
-    v[i] = exp2_fast(fmaf(row.value(i), kLog2e, shift));
+    v[i] = exp2_fast((row.value(i) - top) * kLog2e);
     sum += v[i];
   }
   return 1.0f / group_sum<G>(sum);

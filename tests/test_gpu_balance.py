@@ -252,3 +252,19 @@ def test_recomputed_under_a_checkpoint():
     b = [x.detach().requires_grad_() for x in xs]
     checkpoint(lambda *y: mb.balance_loss(y, 2)[0], *b, use_reentrant=False).backward()
     assert all(torch.equal(x.grad, y.grad) for x, y in zip(a, b))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_rows_of_very_large_and_very_low_logits(dtype):
+    """A row whose mask of the type's lowest value leaves nothing has equal probabilities; beside a logit of 1e10 or more
+    only its equals have any."""
+    x = make(1, 90, 24, dtype)[0]
+    x[3] = torch.finfo(dtype).min
+    x[7] = -1e10
+    x[11] = 1e10
+    x[12, 5:] = torch.finfo(dtype).min
+    x[17] = torch.finfo(dtype).min
+    x[17, 9] = torch.finfo(dtype).max
+    x[23, ::2] = 3e12
+    check([x], 5)
+    check([x[:, :8].contiguous()], 2)
