@@ -21,8 +21,9 @@
 // it, 1.3 TB/s), backward 43 us (4.7 TB/s); the rounds took 174 us forward.
 //
 // The probabilities' sums stay in registers over a group's tokens and are joined per CTA in float32; the CTAs' sums
-// are added as 64-bit whole numbers of 2^-36, whose order does not matter, and the last CTA to finish works out the
-// loss and the gradient's coefficients.
+// are added as 64-bit whole numbers of 2^-36, whose order does not matter, with what a sum has below that (only sums
+// under 2^-12 have any: 24 bits) in units of 2^-90 beside it, so that experts with hardly any probability keep theirs.
+// The last CTA to finish works out the loss and the gradient's coefficients.
 #include "common.cuh"
 #include "host.hpp"
 
@@ -35,6 +36,8 @@ constexpr int MAX_LAYERS = 128;
 constexpr int MAX_EXPERTS = 1024;
 constexpr int CTAS_PER_SM = 2;
 constexpr double kUnit = 68719476736.0;  // 2^36: sums of up to 2^28 probabilities fit 64 bits
+constexpr double kFine = 18014398509481984.0;  // 2^54 to a unit: less than one of each of up to 2^9 CTAs fits 64 bits
+constexpr int MOST_CTAS = 512;
 constexpr int64_t kMostTokens = int64_t(1) << 27;
 
 struct Layers {
@@ -47,8 +50,8 @@ struct Params {
   int64_t tokens;
   const uint8_t* mask;              // per token, or null
   unsigned long long* counts;       // (layers, experts), zero at the start
-  unsigned long long* mass;         // (experts): in units of 2^-36; then the unmasked tokens, the CTAs done and whether
-                                    // a sum was not finite (zero at the start)
+  unsigned long long* mass;         // (2, experts): in units of 2^-36, and what is below them in units of 2^-90; then the
+                                    // unmasked tokens, the CTAs done, whether a sum was not finite (zero at the start)
   float* loss;
   float* coef;                      // E / N^2 (c_e - mean c)
   const float* upstream;
@@ -383,10 +386,15 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) forward(const __grid_con
     float t = 0.f;
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) t += shared[w * p.experts + e];
-    if (t <= 3.4e38f) atomicAdd(p.mass + e, static_cast<unsigned long long>(__double2ll_rn(static_cast<double>(t) * kUnit)));
-    else atomicExch(p.mass + p.experts + 2, 1ull);
+    if (t <= 3.4e38f) {
+      const double units = static_cast<double>(t) * kUnit, whole = floor(units);
+      atomicAdd(p.mass + e, static_cast<unsigned long long>(whole));
+      if (units != whole) atomicAdd(p.mass + p.experts + e, __double2ull_rn((units - whole) * kFine));
+    } else {
+      atomicExch(p.mass + 2 * p.experts + 2, 1ull);
+    }
   }
-  unsigned long long* const said = p.mass + p.experts;  // the unmasked tokens, the CTAs done, a sum not finite
+  unsigned long long* const said = p.mass + 2 * p.experts;  // the unmasked tokens, the CTAs done, a sum not finite
   if (threadIdx.x == 0) atomicAdd(said, static_cast<unsigned long long>(seen));
   __threadfence();
   __syncthreads();
@@ -402,7 +410,8 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) forward(const __grid_con
     for (int l = 0; l < p.layers; ++l) c += __ldcg(p.counts + static_cast<int64_t>(l) * p.experts + e);
     chosen[e] = static_cast<double>(c);
     total += chosen[e];
-    both += chosen[e] * static_cast<double>(__ldcg(p.mass + e));
+    both += chosen[e] * (static_cast<double>(__ldcg(p.mass + e)) +
+                         static_cast<double>(__ldcg(p.mass + p.experts + e)) / kFine);
   }
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) {
@@ -460,7 +469,7 @@ template <typename T, int G, int PER, bool VEC>
 static int launch(const Layers& L, const Params& p, bool back, int sms, cudaStream_t s) {
   constexpr int GROUPS = THREADS / G;
   const int64_t all = (p.tokens + GROUPS - 1) / GROUPS * p.layers;
-  const int64_t most = static_cast<int64_t>(sms) * CTAS_PER_SM;
+  const int64_t most = static_cast<int64_t>(sms) * CTAS_PER_SM < MOST_CTAS ? sms * CTAS_PER_SM : MOST_CTAS;
   const unsigned n = static_cast<unsigned>(all < 1 ? 1 : (all < most ? all : most));
   if (back) backward<T, G, PER, VEC><<<n, THREADS, 0, s>>>(L, p);
   else forward<T, G, PER, VEC><<<n, THREADS, static_cast<size_t>(WARPS) * p.experts * sizeof(float), s>>>(L, p);
@@ -516,7 +525,7 @@ int balance_params(const meep2b_balance* a, const void* const* second, bool back
 extern "C" {
 
 size_t meep2b_balance_workspace_bytes(int32_t experts) {
-  return (static_cast<size_t>(experts) + 3) * sizeof(unsigned long long);
+  return (2 * static_cast<size_t>(experts) + 3) * sizeof(unsigned long long);
 }
 
 int meep2b_balance_loss(const meep2b_balance* a, void* stream) {

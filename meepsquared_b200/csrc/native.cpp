@@ -176,7 +176,11 @@ struct BalanceCall {
   std::vector<const void*> table;
   meep2b_balance args = {};
 
-  // work: the kernel's sums (64-bit words), then the coefficients that the backward pass reads
+  // float32 words of the kernel's sums
+  static int64_t words(int64_t experts) {
+    return static_cast<int64_t>(meep2b_balance_workspace_bytes(static_cast<int32_t>(experts)) / sizeof(float));
+  }
+  // work: the kernel's sums, then the coefficients that the backward pass reads
   BalanceCall(const std::vector<Tensor>& logits, int64_t top_k, const Tensor& mask, const Tensor& work) {
     rows.reserve(logits.size()), table.reserve(logits.size());
     for (const Tensor& x : logits) {
@@ -188,7 +192,7 @@ struct BalanceCall {
     args.tokens = rows[0].size(0), args.top_k = static_cast<int32_t>(top_k), args.dtype = dtype_of(rows[0]);
     args.mask = data<uint8_t>(mask);
     args.workspace = data<void>(work);
-    args.coef = data<float>(work) + 2 * (args.experts + 3);
+    args.coef = data<float>(work) + words(args.experts);
   }
 };
 
@@ -238,7 +242,7 @@ std::tuple<Tensor, Tensor> balance_loss(const std::vector<Tensor>& logits, int64
   const Tensor mask_ = mask.value_or(Tensor());
   {
     const at::NoGradGuard none;
-    work = at::empty({2 * (experts + 3) + experts}, f32);
+    work = at::empty({BalanceCall::words(experts) + experts}, f32);
     loss = at::empty({}, f32);
     const auto i64 = first.options().dtype(at::kLong);
     counts = layers == 1 ? at::empty({experts}, i64) : at::empty({layers, experts}, i64);

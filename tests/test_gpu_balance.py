@@ -268,3 +268,15 @@ def test_rows_of_very_large_and_very_low_logits(dtype):
     x[23, ::2] = 3e12
     check([x], 5)
     check([x[:, :8].contiguous()], 2)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("gap", [10.0, 30.0, 45.0])
+@pytest.mark.parametrize("tokens", [1, 700])
+def test_unlikely_experts_chosen(tokens, gap, dtype):
+    """A choice of experts that have hardly any probability (a given choice need not follow the logits): the loss is a sum
+    of the small ones alone."""
+    x = make(1, tokens, 16, dtype)[0]
+    x[:, 0] += gap
+    ids = torch.arange(tokens, device=DEV)[:, None] % 5 * 3 + torch.tensor([[1, 3]], device=DEV)
+    check([x], 2, ids=[ids])
