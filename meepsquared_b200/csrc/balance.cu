@@ -20,10 +20,11 @@
 // 24 layers of 16,384 x 128 bf16: forward 75 us (112 instructions a token; the integer pipe's minima and maxima bound
 // it, 1.3 TB/s), backward 43 us (4.7 TB/s); the rounds took 174 us forward.
 //
-// The probabilities' sums stay in registers over a group's tokens and are joined per CTA in float32; the CTAs' sums
-// are added as 64-bit whole numbers of 2^-36, whose order does not matter, with what a sum has below that (only sums
-// under 2^-12 have any: 24 bits) in units of 2^-90 beside it, so that experts with hardly any probability keep theirs.
-// The last CTA to finish works out the loss and the gradient's coefficients.
+// The probabilities' sums stay in float32 registers over up to 256 of a group's tokens (equal probabilities, one after
+// another, would be off by 9e-5 of their sum after 7,000) and are joined per CTA in 64 bits; the CTAs' sums are added as
+// 64-bit whole numbers of 2^-36, whose order does not matter, with what a sum has below that in units of 2^-90 beside
+// it (sums under 2^-12, for the most), so that experts with hardly any probability keep theirs. The last CTA to finish
+// works out the loss and the gradient's coefficients.
 #include "common.cuh"
 #include "host.hpp"
 
@@ -38,6 +39,7 @@ constexpr int CTAS_PER_SM = 2;
 constexpr double kUnit = 68719476736.0;  // 2^36: sums of up to 2^28 probabilities fit 64 bits
 constexpr double kFine = 18014398509481984.0;  // 2^54 to a unit: less than one of each of up to 2^9 CTAs fits 64 bits
 constexpr int MOST_CTAS = 512;
+constexpr int FLUSH = 256;  // tokens whose probabilities a lane sums up before they are joined into its CTA's
 constexpr int64_t kMostTokens = int64_t(1) << 27;
 
 struct Layers {
@@ -321,11 +323,13 @@ __device__ __forceinline__ void choose(const Row<float, PER>& row, int lane, int
 
 template <typename T, int G, int PER, bool VEC>
 __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) forward(const __grid_constant__ Layers L, const Params p) {
-  extern __shared__ float shared[];  // WARPS * experts
+  extern __shared__ __align__(8) float shared[];  // WARPS * experts, then `experts` double
   __shared__ int seen;
   __shared__ bool last;
   __shared__ double reduce[2][WARPS];
   int* hist = reinterpret_cast<int*>(shared);  // experts, of the layer in hand
+  double* held = reinterpret_cast<double*>(shared + WARPS * p.experts);  // the CTA's sums of probabilities
+  for (int e = threadIdx.x; e < p.experts; e += THREADS) held[e] = 0.0;
   const int lane = threadIdx.x & (G - 1), warp = threadIdx.x >> 5;
   constexpr int GROUPS = THREADS / G;
   const int group = threadIdx.x / G;
@@ -335,10 +339,29 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) forward(const __grid_con
   const int64_t rounds = (p.tokens + GROUPS - 1) / GROUPS;  // of a layer, a token a group
   const int64_t all = rounds * p.layers;
   const int64_t r0 = all * blockIdx.x / gridDim.x, r1 = all * (blockIdx.x + 1) / gridDim.x;
-  int64_t r = r0;
+  // the sums of probabilities in registers joined into the CTA's: the groups of a warp, then the warps, in order
+  auto join_mass = [&]() {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+#pragma unroll
+      for (int off = G; off < 32; off <<= 1) mass[i] += __shfl_xor_sync(0xffffffffu, mass[i], off);
+      const int e = (i / 8 * G + lane) * 8 + i % 8;
+      if ((threadIdx.x & 31) < G && e < p.experts) shared[warp * p.experts + e] = mass[i];
+      mass[i] = 0.f;
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < p.experts; e += THREADS) {
+      float t = 0.f;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) t += shared[w * p.experts + e];
+      held[e] += static_cast<double>(t);
+    }
+    __syncthreads();
+  };
+  int64_t r = r0, flush = r0 + FLUSH;
   while (r < r1) {
     const int layer = static_cast<int>(r / rounds);
-    const int64_t end = min(r1, (layer + 1) * rounds);
+    const int64_t end = min(min(r1, (layer + 1) * rounds), flush);
     const T* logits = static_cast<const T*>(L.logits[layer]);
     const int64_t* ids = static_cast<const int64_t*>(L.other[layer]);
     for (int e = threadIdx.x; e < p.experts; e += THREADS) hist[e] = 0;
@@ -371,23 +394,13 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) forward(const __grid_con
     for (int e = threadIdx.x; e < p.experts; e += THREADS)
       if (hist[e]) atomicAdd(p.counts + static_cast<int64_t>(layer) * p.experts + e, static_cast<unsigned long long>(hist[e]));
     __syncthreads();
+    if (r == flush && r < r1) join_mass(), flush += FLUSH;
   }
-  // the CTA's sums: the groups of a warp, then the warps, in order
   if (live) atomicAdd(&seen, live);
-#pragma unroll
-  for (int i = 0; i < PER; ++i) {
-#pragma unroll
-    for (int off = G; off < 32; off <<= 1) mass[i] += __shfl_xor_sync(0xffffffffu, mass[i], off);
-    const int e = (i / 8 * G + lane) * 8 + i % 8;
-    if ((threadIdx.x & 31) < G && e < p.experts) shared[warp * p.experts + e] = mass[i];
-  }
-  __syncthreads();
-  for (int e = threadIdx.x; e < p.experts; e += THREADS) {
-    float t = 0.f;
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w) t += shared[w * p.experts + e];
-    if (t <= 3.4e38f) {
-      const double units = static_cast<double>(t) * kUnit, whole = floor(units);
+  join_mass();
+  for (int e = threadIdx.x; e < p.experts; e += THREADS) {  // (this thread's own of held)
+    const double units = held[e] * kUnit, whole = floor(units);
+    if (units < 1.8e19) {
       atomicAdd(p.mass + e, static_cast<unsigned long long>(whole));
       if (units != whole) atomicAdd(p.mass + p.experts + e, __double2ull_rn((units - whole) * kFine));
     } else {
@@ -472,7 +485,7 @@ static int launch(const Layers& L, const Params& p, bool back, int sms, cudaStre
   const int64_t most = static_cast<int64_t>(sms) * CTAS_PER_SM < MOST_CTAS ? sms * CTAS_PER_SM : MOST_CTAS;
   const unsigned n = static_cast<unsigned>(all < 1 ? 1 : (all < most ? all : most));
   if (back) backward<T, G, PER, VEC><<<n, THREADS, 0, s>>>(L, p);
-  else forward<T, G, PER, VEC><<<n, THREADS, static_cast<size_t>(WARPS) * p.experts * sizeof(float), s>>>(L, p);
+  else forward<T, G, PER, VEC><<<n, THREADS, (WARPS * sizeof(float) + sizeof(double)) * p.experts, s>>>(L, p);
   return launch_status();
 }
 

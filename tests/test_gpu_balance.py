@@ -280,3 +280,13 @@ def test_unlikely_experts_chosen(tokens, gap, dtype):
     x[:, 0] += gap
     ids = torch.arange(tokens, device=DEV)[:, None] % 5 * 3 + torch.tensor([[1, 3]], device=DEV)
     check([x], 2, ids=[ids])
+
+
+@pytest.mark.parametrize("experts,tokens", [(100, 1 << 26), (7, 1 << 27)])
+def test_many_tokens_of_equal_probabilities(experts, tokens):
+    """Every probability is 1 / E and the loss exactly top_k, whatever the choice: float32 sums of thousands of equal
+    summands drift, all in one direction."""
+    x = torch.zeros((tokens, experts), dtype=torch.bfloat16, device=DEV)
+    loss, counts = mb.balance_loss(x, 3)
+    assert counts[:3].tolist() == [tokens] * 3 and not counts[3:].any()
+    assert abs(float(loss) - 3.0) <= 1e-5 * 3.0
