@@ -915,7 +915,8 @@ __global__ void __launch_bounds__(256) vocab_finish(const float* __restrict__ ac
   const int parts = state[kParts];
   const float g = row_upstream(upstream, per_token, mean, static_cast<int>(t), live);
   const float own = target_gradient(rows.miss[row], g);
-  const float a = rounded ? 1.f : g * rows.scale[row];
+  // scale and g apart: a row whose Z is near 2^96 times a small g is below float32's normal numbers
+  const float scale = rounded ? 1.f : rows.scale[row], a = rounded ? 1.f : g;
   const float b = rounded ? own - bf16_round(own) : own;
   const int y = target[row];
   const uint4* wr = reinterpret_cast<const uint4*>(weight + static_cast<int64_t>(y < 0 ? 0 : y) * ld_weight);
@@ -937,10 +938,10 @@ __global__ void __launch_bounds__(256) vocab_finish(const float* __restrict__ ac
       v[4] += w[s].x, v[5] += w[s].y, v[6] += w[s].z, v[7] += w[s].w;
     }
   }
-  v[0] = a * v[0] + b * bf16_lo(k.x), v[1] = a * v[1] + b * bf16_hi(k.x);
-  v[2] = a * v[2] + b * bf16_lo(k.y), v[3] = a * v[3] + b * bf16_hi(k.y);
-  v[4] = a * v[4] + b * bf16_lo(k.z), v[5] = a * v[5] + b * bf16_hi(k.z);
-  v[6] = a * v[6] + b * bf16_lo(k.w), v[7] = a * v[7] + b * bf16_hi(k.w);
+  v[0] = a * (scale * v[0]) + b * bf16_lo(k.x), v[1] = a * (scale * v[1]) + b * bf16_hi(k.x);
+  v[2] = a * (scale * v[2]) + b * bf16_lo(k.y), v[3] = a * (scale * v[3]) + b * bf16_hi(k.y);
+  v[4] = a * (scale * v[4]) + b * bf16_lo(k.z), v[5] = a * (scale * v[5]) + b * bf16_hi(k.z);
+  v[6] = a * (scale * v[6]) + b * bf16_lo(k.w), v[7] = a * (scale * v[7]) + b * bf16_hi(k.w);
   to[i] = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
                      pack_bf16x2(v[6], v[7]));
 }

@@ -398,3 +398,24 @@ def test_two_streams_at_once():
     for i, result in enumerate(got):
         assert all(torch.equal(x, y) for x, y in zip(result, want[i % 2]))
     assert _lib.device_error(0) == 0
+
+
+def test_a_small_upstream_gradient_on_far_targets():
+    """Logits near, but within, the window above the target (about 2^90), times an upstream gradient of 1e-15 or so: the
+    row's scale times the gradient alone would be below float32's normal range, the hidden states' gradient is not."""
+    gen = torch.Generator().manual_seed(11)
+    vocab, hidden = 600, 64
+    w = (torch.randn((vocab, hidden), generator=gen) * 0.02).to(DEV, torch.bfloat16)
+    w[:, 0] = 0.0
+    w[-1, 0] = 1.0  # its logit is the first component of the hidden state
+    h = torch.randn((40, hidden), generator=gen).to(DEV, torch.bfloat16)
+    h[:, 0] = torch.linspace(58.0, 64.0, 40)
+    t = torch.randint(0, vocab - 1, (40,), generator=gen).to(DEV)
+    for g in (1e-12, 1e-15, 1e-17, 1e-20):
+        up = torch.full((40,), g, device=DEV)
+        losses, dh, _, tol, tol_h, _ = formula(h, w, t, up)
+        leaf = h.detach().requires_grad_()
+        loss = mb.linear_cross_entropy(leaf, w, t, reduction="none")
+        within(loss, losses, tol, "losses")
+        loss.backward(up)
+        within(leaf.grad, dh, tol_h, f"dh at {g}")
