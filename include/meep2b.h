@@ -473,7 +473,7 @@ typedef struct meep2b_head_norm {
   int64_t k_stride[3];
   int32_t dtype;
   int32_t angle_dtype;
-  const void* q_weight;         /* (dim), as q */
+  const void* q_weight;         /* (dim), as q, or float32 (weight_f32) */
   const void* k_weight;
   const void* cos;
   const void* sin;
@@ -482,13 +482,14 @@ typedef struct meep2b_head_norm {
   int64_t angles;
   const int64_t* positions;
   float eps;
+  int32_t weight_f32;           /* nonzero: both weights, and their gradients, are float32 beside bf16 heads */
   void* q_out;                  /* forward: the outputs; backward: the gradients of q and k */
   void* k_out;
   const void* dq_out;           /* backward: the outputs' gradients */
   const void* dk_out;
   int64_t dq_out_stride[3];
   int64_t dk_out_stride[3];
-  void* dq_weight;              /* backward: the weights' gradients, or both NULL */
+  void* dq_weight;              /* backward: the weights' gradients, in the weights' type, or both NULL */
   void* dk_weight;
   float* partial;               /* backward, with them: meep2b_head_norm_partials() * dim */
 } meep2b_head_norm;

@@ -15,10 +15,11 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_wei
 
     y = R(pos) (x / sqrt(mean(x^2) + eps) * weight), float32 inside and one rounding at the end. bf16 or float32 (both
     alike), any strides (slices of a fused projection are read in place where they start on 16 bytes); D a multiple of
-    16 up to 256. q_weight, k_weight (D). cos, sin (P, n), float32 or bf16: row p holds the angles of position p; the
-    first 2n dimensions turn in pairs (i, i + n), the others stay (n a multiple of 8, 2n <= D). positions (B, T)
-    integers, or None: 0 .. T - 1 in every sequence (P >= T). A position outside the angles makes its turned values
-    NaN. The results are contiguous (B, T, heads, D). Differentiable in q, k and the weights (once)."""
+    16 up to 256. q_weight, k_weight (D): both of the heads' type, or read as float32; a weight's gradient is rounded
+    once, to the weight's type. cos, sin (P, n), float32 or bf16: row p holds the angles of position p; the first 2n
+    dimensions turn in pairs (i, i + n), the others stay (n a multiple of 8, 2n <= D). positions (B, T) integers, or
+    None: 0 .. T - 1 in every sequence (P >= T). A position outside the angles makes its turned values NaN. The results
+    are contiguous (B, T, heads, D). Differentiable in q, k and the weights (once)."""
     if not q.is_cuda:
         raise RuntimeError("qk_norm_rope runs on a CUDA GPU")
     qs, ks, cs = q.shape, k.shape, cos.shape

@@ -78,7 +78,7 @@ class HeadNorm(ctypes.Structure):
         ("q", _p), ("k", _p), ("batch", _i64), ("length", _i64), ("q_heads", _i32), ("kv_heads", _i32),
         ("dim", _i32), ("half", _i32), ("q_stride", _i64 * 3), ("k_stride", _i64 * 3), ("dtype", _i32),
         ("angle_dtype", _i32), ("q_weight", _p), ("k_weight", _p), ("cos", _p), ("sin", _p), ("ld_cos", _i64),
-        ("ld_sin", _i64), ("angles", _i64), ("positions", _p), ("eps", _f32), ("q_out", _p), ("k_out", _p),
+        ("ld_sin", _i64), ("angles", _i64), ("positions", _p), ("eps", _f32), ("weight_f32", _i32), ("q_out", _p), ("k_out", _p),
         ("dq_out", _p), ("dk_out", _p), ("dq_out_stride", _i64 * 3), ("dk_out_stride", _i64 * 3),
         ("dq_weight", _p), ("dk_weight", _p), ("partial", _p),
     ]

@@ -118,8 +118,30 @@ struct Ring {
   static constexpr int BYTES = DEPTH * CHUNKS * THREADS * 16;
 };
 
-// T: the heads' type; A: the angles'; G: lanes a head; BACKWARD; DW: the weights' gradients too.
-template <typename T, typename A, int G, bool BACKWARD, bool DW>
+// A chunk's norm weights as they are stored (half the registers in bf16), widened at each use.
+template <typename W, int N>
+struct Weights {
+  static constexpr int WORDS = N / Vec<W>::N;
+  uint4 w[WORDS];
+  __device__ __forceinline__ void load(const void* base, int at) {
+    const uint4* from = reinterpret_cast<const uint4*>(static_cast<const W*>(base) + at);
+#pragma unroll
+    for (int i = 0; i < WORDS; ++i) w[i] = from[i];
+  }
+  __device__ __forceinline__ void unpack(float (&v)[N]) const {
+#pragma unroll
+    for (int i = 0; i < WORDS; ++i) {
+      float part[Vec<W>::N];
+      Vec<W>::unpack(w[i], part);
+#pragma unroll
+      for (int j = 0; j < Vec<W>::N; ++j) v[i * Vec<W>::N + j] = part[j];
+    }
+  }
+};
+
+// T: the heads' type; W: the norm weights' (T or float); A: the angles'; G: lanes a head; BACKWARD; DW: the weights'
+// gradients too.
+template <typename T, typename W, typename A, int G, bool BACKWARD, bool DW>
 __global__ void __launch_bounds__(THREADS, BACKWARD ? 2 : 3) norm_rotate(const Params p) {
   constexpr int N = Vec<T>::N;
   using R = Ring<BACKWARD>;
@@ -136,11 +158,8 @@ __global__ void __launch_bounds__(THREADS, BACKWARD ? 2 : 3) norm_rotate(const P
   const int c0 = turns ? lane : 2 * turned + 2 * (lane - turned), c1 = turns ? lane + turned : c0 + 1;
   const int o0 = c0 * N, o1 = c1 * N;
   float dw0[N] = {}, dw1[N] = {};
-  uint4 wr0 = make_uint4(0, 0, 0, 0), wr1 = wr0;  // the weight as it is stored: half the registers in bf16
-  if (here) {
-    wr0 = *reinterpret_cast<const uint4*>(static_cast<const T*>(s.weight) + o0);
-    wr1 = *reinterpret_cast<const uint4*>(static_cast<const T*>(s.weight) + o1);
-  }
+  Weights<W, N> wr0 = {}, wr1 = {};
+  if (here) wr0.load(s.weight, o0), wr1.load(s.weight, o1);
   // items fit 31 bits (the entry point's limit on tokens x heads), and a stride more 32
   const int span = s.span;
   const uint32_t spans = (s.heads + span - 1) / span;
@@ -232,7 +251,7 @@ __global__ void __launch_bounds__(THREADS, BACKWARD ? 2 : 3) norm_rotate(const P
 #pragma unroll
     for (int off = G / 2; off > 0; off >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, off);
     const float r = rsqrtf(fmaf(sq, inv_dim, p.eps));
-    Vec<T>::unpack(wr0, w0), Vec<T>::unpack(wr1, w1);
+    wr0.unpack(w0), wr1.unpack(w1);
     if (!BACKWARD) {
 #pragma unroll
       for (int j = 0; j < N; ++j) {
@@ -317,11 +336,11 @@ __global__ void __launch_bounds__(1024) join_weight(const float* __restrict__ pa
   }
 }
 
-template <typename T, typename A, bool BACKWARD, bool DW>
+template <typename T, typename W, typename A, bool BACKWARD, bool DW>
 static void launch(const Params& p, unsigned blocks, cudaStream_t s) {
   const int slots = p.dim / (2 * Vec<T>::N);  // lanes a head needs
 #define MEEP2B_HEADS(G)                                                                                      \
-  norm_rotate<T, A, G, BACKWARD, DW><<<blocks, THREADS, Ring<BACKWARD>::BYTES, s>>>(p)
+  norm_rotate<T, W, A, G, BACKWARD, DW><<<blocks, THREADS, Ring<BACKWARD>::BYTES, s>>>(p)
   if (slots <= 1) MEEP2B_HEADS(1);
   else if (slots <= 2) MEEP2B_HEADS(2);
   else if (slots <= 4) MEEP2B_HEADS(4);
@@ -331,15 +350,17 @@ static void launch(const Params& p, unsigned blocks, cudaStream_t s) {
 #undef MEEP2B_HEADS
 }
 
+template <typename T, typename W, bool BACKWARD, bool DW>
+static void launch_angles(const Params& p, int angle_dtype, unsigned blocks, cudaStream_t s) {
+  if (angle_dtype == MEEP2B_BF16) launch<T, W, __nv_bfloat16, BACKWARD, DW>(p, blocks, s);
+  else launch<T, W, float, BACKWARD, DW>(p, blocks, s);
+}
+
 template <bool BACKWARD, bool DW>
-static void launch_types(const Params& p, int dtype, int angle_dtype, unsigned blocks, cudaStream_t s) {
-  if (dtype == MEEP2B_BF16) {
-    if (angle_dtype == MEEP2B_BF16) launch<__nv_bfloat16, __nv_bfloat16, BACKWARD, DW>(p, blocks, s);
-    else launch<__nv_bfloat16, float, BACKWARD, DW>(p, blocks, s);
-  } else {
-    if (angle_dtype == MEEP2B_BF16) launch<float, __nv_bfloat16, BACKWARD, DW>(p, blocks, s);
-    else launch<float, float, BACKWARD, DW>(p, blocks, s);
-  }
+static void launch_types(const Params& p, const meep2b_head_norm* a, unsigned blocks, cudaStream_t s) {
+  if (a->dtype == MEEP2B_F32) launch_angles<float, float, BACKWARD, DW>(p, a->angle_dtype, blocks, s);
+  else if (a->weight_f32) launch_angles<__nv_bfloat16, float, BACKWARD, DW>(p, a->angle_dtype, blocks, s);
+  else launch_angles<__nv_bfloat16, __nv_bfloat16, BACKWARD, DW>(p, a->angle_dtype, blocks, s);
 }
 
 // How the heads of a token are taken: up to 8 in a row, fewer while that leaves groups without work, in runs of about
@@ -428,7 +449,7 @@ int meep2b_head_norm_rotate(const meep2b_head_norm* a, void* stream) {
   int sms = 0;
   MEEP2B_TRY(device_sms(&sms));
   const int64_t blocks = head_norm::shape(p, head_norm::lanes_of(p.dim, a->dtype), sms, INT32_MAX);
-  head_norm::launch_types<false, false>(p, a->dtype, a->angle_dtype, static_cast<unsigned>(blocks), s);
+  head_norm::launch_types<false, false>(p, a, static_cast<unsigned>(blocks), s);
   return launch_status();
 }
 
@@ -446,13 +467,13 @@ int meep2b_head_norm_rotate_backward(const meep2b_head_norm* a, void* stream) {
     MEEP2B_TRY(device_sms(&sms));
     const int64_t most = !dw ? INT32_MAX : (2 * sms < head_norm::MAX_PARTIALS ? 2 * sms : head_norm::MAX_PARTIALS);
     blocks = static_cast<int>(head_norm::shape(p, head_norm::lanes_of(p.dim, a->dtype), sms, most));
-    if (dw) head_norm::launch_types<true, true>(p, a->dtype, a->angle_dtype, blocks, s);
-    else head_norm::launch_types<true, false>(p, a->dtype, a->angle_dtype, blocks, s);
+    if (dw) head_norm::launch_types<true, true>(p, a, blocks, s);
+    else head_norm::launch_types<true, false>(p, a, blocks, s);
     MEEP2B_TRY(launch_status());
   }
   if (dw) {
     const dim3 grid((p.dim + 31) / 32, 2);
-    if (a->dtype == MEEP2B_BF16)
+    if (a->dtype == MEEP2B_BF16 && !a->weight_f32)
       head_norm::join_weight<<<grid, 1024, 0, s>>>(p.partial, p.q_blocks, blocks, p.dim,
                                                    static_cast<__nv_bfloat16*>(a->dq_weight),
                                                    static_cast<__nv_bfloat16*>(a->dk_weight));

@@ -76,6 +76,11 @@ Tensor heads(const Tensor& t) {
   return s[3] == 1 && s[0] % vec == 0 && s[1] % vec == 0 && s[2] % vec == 0 && aligned(t) ? t : dense(t);
 }
 
+// The type the norm weights are read in: the heads' own where both have it, else float32, which holds every other.
+at::ScalarType weight_type(const Tensor& x, const Tensor& wq, const Tensor& wk) {
+  return wq.scalar_type() == x.scalar_type() && wk.scalar_type() == x.scalar_type() ? x.scalar_type() : at::kFloat;
+}
+
 Tensor vector_as(const Tensor& w, at::ScalarType type) {
   Tensor v = w.scalar_type() == type ? w : w.to(type);
   return v.is_contiguous() && aligned(v) ? v : dense(v);
@@ -87,14 +92,15 @@ struct HeadsCall {
 
   HeadsCall(const Tensor& q_, const Tensor& k_, const Tensor& wq_, const Tensor& wk_, const Tensor& cos_,
             const Tensor& sin_, const Tensor& positions_, double eps)
-      : q(heads(q_)), k(heads(k_)), wq(vector_as(wq_, q_.scalar_type())), wk(vector_as(wk_, q_.scalar_type())),
-        cos(cos_), sin(sin_), positions(positions_) {
+      : q(heads(q_)), k(heads(k_)), wq(vector_as(wq_, weight_type(q_, wq_, wk_))),
+        wk(vector_as(wk_, weight_type(q_, wq_, wk_))), cos(cos_), sin(sin_), positions(positions_) {
     args.q = data<void>(q), args.k = data<void>(k);
     args.batch = q.size(0), args.length = q.size(1);
     args.q_heads = static_cast<int32_t>(q.size(2)), args.kv_heads = static_cast<int32_t>(k.size(2));
     args.dim = static_cast<int32_t>(q.size(3)), args.half = static_cast<int32_t>(cos.size(1));
     for (int i = 0; i < 3; ++i) args.q_stride[i] = q.stride(i), args.k_stride[i] = k.stride(i);
     args.dtype = dtype_of(q), args.angle_dtype = dtype_of(cos);
+    args.weight_f32 = wq.scalar_type() == at::kFloat;
     args.q_weight = data<void>(wq), args.k_weight = data<void>(wk);
     args.cos = data<void>(cos), args.sin = data<void>(sin);
     args.ld_cos = cos.stride(0), args.ld_sin = sin.stride(0), args.angles = cos.size(0);

@@ -306,3 +306,34 @@ def test_recomputed_under_a_checkpoint():
     out = checkpoint(lambda *y: mb.qk_norm_rope(*y, cos, sin), *b, use_reentrant=False)
     got = torch.autograd.grad(out, b, list(parts[4:]))
     assert all(torch.equal(x, y) for x, y in zip(want, got))
+
+
+@pytest.mark.parametrize("kinds", [(torch.float32, torch.float32), (torch.float32, torch.bfloat16),
+                                   (torch.bfloat16, torch.float16), (torch.float16, torch.float32)],
+                         ids=["f32-f32", "f32-bf16", "bf16-f16", "f16-f32"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("dim,half", [(16, 8), (64, 16), (80, 40), (128, 64), (256, 128)])
+def test_weights_of_their_own_type(dim, half, dtype, kinds):
+    """Norm weights that the heads' type cannot hold: used as they are, and each gradient rounded to its weight's type
+    alone (float16 has 11 significant bits, normal from 2^-14)."""
+    bits = {torch.float32: U, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+    q, k, _, _, dq, dk = make(3, 37, 5, 2, dim, dtype)
+    gen = torch.Generator().manual_seed(9)
+    ws = [(1 + 0.2 * torch.randn((dim,), generator=gen)).to(DEV, kind) for kind in kinds]
+    assert dtype == torch.float32 or any(bool((w.to(dtype) != w).any()) for w in ws)
+    cos, sin = angles(37, half)
+    at = torch.arange(37, device=DEV).expand(3, 37)
+    c, s = cos.double()[at][:, :, None], sin.double()[at][:, :, None]
+    leaves = [x.detach().requires_grad_() for x in (q, k, *ws)]
+    out = mb.qk_norm_rope(*leaves, cos, sin)
+    grads = torch.autograd.grad(out, leaves, [dq, dk])
+    for i, (x, w, dy) in enumerate(((q, ws[0], dq), (k, ws[1], dk))):
+        y, dx, (dw, tol) = formula(x, w, c, s, 1e-6, dy)
+        near(out[i].detach(), y, f"out {i}")
+        near(grads[i], dx, f"dx {i}")
+        tol = tol + 1.01 * (bits[w.dtype] - ULP[dtype]) * dw.abs() + (2.0 ** -24 if w.dtype == torch.float16 else 0.0)
+        near(grads[2 + i], (dw, tol), f"dw {i}")
+        assert out[i].dtype == dtype and grads[2 + i].dtype == w.dtype
+    with torch.no_grad():
+        again = mb.qk_norm_rope(q, k, *ws, cos, sin)
+    assert torch.equal(again[0], out[0]) and torch.equal(again[1], out[1])
