@@ -51,4 +51,4 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_wei
         if positions.dtype not in (torch.int64, torch.int32):
             raise TypeError(f"positions in {positions.dtype}: int64 or int32 expected")
         positions = positions.to(torch.int64).contiguous()
-    return _lib.native().qk_norm_rope(q, k, q_weight, k_weight, cos.detach(), sin.detach(), positions, eps)
+    return _lib.native().qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps)

@@ -48,6 +48,12 @@ int32_t dtype_of(const Tensor& t) { return t.scalar_type() == at::kBFloat16 ? ME
 
 bool wants(const Tensor& t) { return at::GradMode::is_enabled() && t.requires_grad(); }
 
+// The nodes know the backward direction alone: a tangent of forward-mode differentiation would be lost without a word.
+void refuse_tangents(const char* name, at::ArrayRef<Tensor> inputs) {
+  for (const Tensor& t : inputs)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(0).defined(), name, " has no forward-mode derivative");
+}
+
 Tensor dense(const Tensor& t) { return t.clone(at::MemoryFormat::Contiguous); }
 
 // The results of a backward pass that was asked to be differentiable itself: an error if they are.
@@ -149,8 +155,10 @@ struct QkNormRopeBackward : torch::autograd::Node {
 };
 
 std::tuple<Tensor, Tensor> qk_norm_rope(const Tensor& q, const Tensor& k, const Tensor& wq, const Tensor& wk,
-                                        const Tensor& cos, const Tensor& sin, const std::optional<Tensor>& positions,
+                                        const Tensor& cos_, const Tensor& sin_, const std::optional<Tensor>& positions,
                                         double eps) {
+  refuse_tangents("qk_norm_rope", {q, k, wq, wk, cos_, sin_});
+  const Tensor cos = cos_.detach(), sin = sin_.detach();
   const c10::cuda::CUDAGuard guard(q.device());
   const bool graph = wants(q) || wants(k) || wants(wq) || wants(wk);
   const Tensor pos = positions.value_or(Tensor());
@@ -238,6 +246,7 @@ struct BalanceLossBackward : torch::autograd::Node {
 
 std::tuple<Tensor, Tensor> balance_loss(const std::vector<Tensor>& logits, int64_t top_k,
                                         const std::optional<Tensor>& mask, const std::vector<Tensor>& index) {
+  refuse_tangents("balance_loss", logits);
   const Tensor& first = logits[0];
   const c10::cuda::CUDAGuard guard(first.device());
   bool graph = false;
@@ -354,6 +363,7 @@ struct LinearCrossEntropyBackward : torch::autograd::Node {
 
 Tensor linear_cross_entropy(const Tensor& hidden, const Tensor& weight, const Tensor& targets, int64_t ignore,
                             int64_t reduction, int64_t piece_cols, int64_t planes) {
+  refuse_tangents("linear_cross_entropy", {hidden, weight});
   const c10::cuda::CUDAGuard guard(hidden.device());
   const bool trained = wants(weight), accumulate = wants(hidden) && !trained;
   Plan plan;

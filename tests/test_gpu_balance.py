@@ -290,3 +290,23 @@ def test_many_tokens_of_equal_probabilities(experts, tokens):
     loss, counts = mb.balance_loss(x, 3)
     assert counts[:3].tolist() == [tokens] * 3 and not counts[3:].any()
     assert abs(float(loss) - 3.0) <= 1e-5 * 3.0
+
+
+@pytest.mark.parametrize("which", [0, 1])
+def test_forward_mode_derivatives_are_refused(which):
+    """An answer without the tangent would read as a derivative of zero."""
+    import torch.autograd.forward_ad as forward
+
+    inputs = make(2, 20, 16, torch.float32)
+
+    def call(*x):
+        return mb.balance_loss(x, 2)[0]
+
+    with forward.dual_level():
+        dual = [forward.make_dual(x, torch.ones_like(x)) if i == which else x for i, x in enumerate(inputs)]
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            call(*dual)
+    with pytest.raises((NotImplementedError, RuntimeError)):
+        torch.func.jvp(lambda x: call(*[x if i == which else y for i, y in enumerate(inputs)]), (inputs[which],),
+                       (torch.ones_like(inputs[which]),))
+    call(*inputs)  # and nothing is left behind

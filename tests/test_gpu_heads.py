@@ -337,3 +337,24 @@ def test_weights_of_their_own_type(dim, half, dtype, kinds):
     with torch.no_grad():
         again = mb.qk_norm_rope(q, k, *ws, cos, sin)
     assert torch.equal(again[0], out[0]) and torch.equal(again[1], out[1])
+
+
+@pytest.mark.parametrize("which", range(6))
+def test_forward_mode_derivatives_are_refused(which):
+    """An answer without the tangent would read as a derivative of zero."""
+    import torch.autograd.forward_ad as forward
+
+    q, k, wq, wk, _, _ = make(1, 6, 2, 1, 64, torch.bfloat16)
+    inputs = (q, k, wq, wk, *angles(6, 32))
+
+    def call(*x):
+        return mb.qk_norm_rope(*x)[0]
+
+    with forward.dual_level():
+        dual = [forward.make_dual(x, torch.ones_like(x)) if i == which else x for i, x in enumerate(inputs)]
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            call(*dual)
+    with pytest.raises((NotImplementedError, RuntimeError)):
+        torch.func.jvp(lambda x: call(*[x if i == which else y for i, y in enumerate(inputs)]), (inputs[which],),
+                       (torch.ones_like(inputs[which]),))
+    call(*inputs)  # and nothing is left behind

@@ -419,3 +419,24 @@ def test_a_small_upstream_gradient_on_far_targets():
         within(loss, losses, tol, "losses")
         loss.backward(up)
         within(leaf.grad, dh, tol_h, f"dh at {g}")
+
+
+@pytest.mark.parametrize("which", [0, 1])
+def test_forward_mode_derivatives_are_refused(which):
+    """An answer without the tangent would read as a derivative of zero."""
+    import torch.autograd.forward_ad as forward
+
+    h, w, t = inputs(20, 64, 100)
+    given = (h, w)
+
+    def call(*x):
+        return mb.linear_cross_entropy(*x, t)
+
+    with forward.dual_level():
+        dual = [forward.make_dual(x, torch.ones_like(x)) if i == which else x for i, x in enumerate(given)]
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            call(*dual)
+    with pytest.raises((NotImplementedError, RuntimeError)):
+        torch.func.jvp(lambda x: call(*[x if i == which else y for i, y in enumerate(given)]), (given[which],),
+                       (torch.ones_like(given[which]),))
+    call(*given)  # and nothing is left behind
