@@ -148,18 +148,24 @@ def _attention_forward(self, hidden_states, position_embeddings, attention_mask=
     return self.o_proj(out.transpose(1, 2).reshape(batch, length, -1)), None
 
 
+def _check_attention(name, module):
+    """Refuses an attention module that _attention_forward does not compute."""
+    if getattr(module, "sliding_window", None) is not None:
+        raise NotImplementedError(f"{name}: attention within a sliding window")
+    if module.q_norm.variance_epsilon != module.k_norm.variance_epsilon:
+        raise NotImplementedError(f"{name}: norms of different epsilon")
+
+
 def install_attention(model) -> int:
     """qk_norm_rope in every attention module with normed heads (Transformers' Qwen3 layout: rotary pairs (i, i + n),
-    torch's scaled_dot_product_attention behind it); returns how many were patched."""
-    patched = 0
-    for name, module in attention_modules(model):
-        if getattr(module, "sliding_window", None) is not None:
-            raise NotImplementedError(f"{name}: attention within a sliding window")
-        if module.q_norm.variance_epsilon != module.k_norm.variance_epsilon:
-            raise NotImplementedError(f"{name}: norms of different epsilon")
+    torch's scaled_dot_product_attention behind it); returns how many were patched. Raises NotImplementedError, with none
+    patched, if there is one that cannot be."""
+    found = list(attention_modules(model))
+    for name, module in found:  # all of them before the first is changed
+        _check_attention(name, module)
+    for _, module in found:
         module.forward = types.MethodType(_attention_forward, module)
-        patched += 1
-    return patched
+    return len(found)
 
 
 def _routers(model):

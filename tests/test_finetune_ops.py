@@ -96,3 +96,17 @@ def test_bad_arguments_are_refused_before_anything_runs():
         bad = _lib.HeadNorm.from_buffer_copy(heads)
         setattr(bad, field, value)
         assert lib.meep2b_head_norm_rotate(ctypes.byref(bad), None) == status, field
+
+
+@pytest.mark.parametrize("spoil", [lambda a: setattr(a, "sliding_window", 128),
+                                   lambda a: setattr(a.k_norm, "variance_epsilon", 1e-5)], ids=["window", "epsilon"])
+def test_a_refused_module_leaves_the_others_as_they_were(spoil):
+    from test_model import tiny_qwen3_moe
+
+    model = tiny_qwen3_moe(layers=3)
+    found = [a for _, a in mb.model.attention_modules(model)]
+    before = [a.forward for a in found]
+    spoil(found[-1])
+    with pytest.raises(NotImplementedError):
+        mb.model.install_attention(model)
+    assert [a.forward for a in found] == before
