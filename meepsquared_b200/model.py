@@ -121,8 +121,24 @@ def attention_modules(model):
             yield name, module
 
 
+def _attention_implementation(module):
+    """The attention that the module is configured for, or an error where it is one whose masks say something else.
+
+    torch's attention and the plain one get every boundary as a (batch, 1, queries, keys) mask, and causal attention alone
+    as none; the others take packed sequences without a mask, from the positions or from cu_seq_lens."""
+    name = getattr(getattr(module, "config", None), "_attn_implementation", None)
+    if name not in (None, "sdpa", "eager"):
+        raise NotImplementedError(f"attention implementation {name!r}: load the model with attn_implementation='sdpa'")
+    return name
+
+
 def _attention_forward(self, hidden_states, position_embeddings, attention_mask=None, past_key_values=None, **kwargs):
     """The attention's forward with norms and rotation in one pass between the projections and torch's attention."""
+    implementation = _attention_implementation(self)  # (it may have been changed since install_attention)
+    if attention_mask is None and any(kwargs.get(n) is not None for n in ("cu_seq_lens_q", "cu_seq_lens_k")):
+        raise NotImplementedError("packed sequences (cu_seq_lens) need an attention mask that separates them")
+    if implementation == "eager" and (kwargs.get("output_attentions") or getattr(self.config, "output_attentions", False)):
+        raise NotImplementedError("attention weights (output_attentions) are not computed")
     batch, length = hidden_states.shape[:2]
     heads = (batch, length, -1, self.head_dim)
     q, k, v = (f(hidden_states).view(heads) for f in (self.q_proj, self.k_proj, self.v_proj))
@@ -150,6 +166,7 @@ def _attention_forward(self, hidden_states, position_embeddings, attention_mask=
 
 def _check_attention(name, module):
     """Refuses an attention module that _attention_forward does not compute."""
+    _attention_implementation(module)
     if getattr(module, "sliding_window", None) is not None:
         raise NotImplementedError(f"{name}: attention within a sliding window")
     if module.q_norm.variance_epsilon != module.k_norm.variance_epsilon:

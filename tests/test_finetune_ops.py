@@ -110,3 +110,58 @@ def test_a_refused_module_leaves_the_others_as_they_were(spoil):
     with pytest.raises(NotImplementedError):
         mb.model.install_attention(model)
     assert [a.forward for a in found] == before
+
+
+def plain_qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions=None, eps=1e-6):
+    """qk_norm_rope in elementary operations, for what can be said of a patched attention without a GPU."""
+    at = torch.arange(q.shape[1]).expand(q.shape[:2]) if positions is None else positions
+    c, s, n = cos[at][:, :, None], sin[at][:, :, None], cos.shape[1]
+
+    def heads(x, w):
+        x = x * (x.square().mean(-1, keepdim=True) + eps).rsqrt() * w
+        a, b = x[..., :n], x[..., n:2 * n]
+        return torch.cat([a * c - b * s, b * c + a * s, x[..., 2 * n:]], -1)
+
+    return heads(q, q_weight), heads(k, k_weight)
+
+
+@pytest.mark.parametrize("implementation", ["flash_attention_2", "flex_attention", "paged|sdpa"])
+def test_attention_that_separates_sequences_without_a_mask_is_refused(implementation):
+    """A model for flash attention gets packed sequences without a mask: taken for causal attention, tokens would see other
+    sequences."""
+    from test_model import tiny_qwen3_moe
+
+    model = tiny_qwen3_moe()
+    model.config._attn_implementation = implementation
+    with pytest.raises(NotImplementedError, match="attn_implementation"):
+        mb.model.install_attention(model)
+    model.config._attn_implementation = "sdpa"
+    mb.model.install_attention(model)
+    model.config._attn_implementation = implementation  # changed afterwards
+    attention = next(mb.model.attention_modules(model))[1]
+    x, angles = torch.zeros((1, 4, 256)), (torch.ones((1, 4, 64)), torch.zeros((1, 4, 64)))
+    with pytest.raises(NotImplementedError, match="attn_implementation"):
+        attention(x, position_embeddings=angles, attention_mask=None)
+
+
+def test_packed_sequences_and_attention_weights(monkeypatch):
+    from test_model import tiny_qwen3_moe
+
+    model = tiny_qwen3_moe().eval()
+    ids = torch.randint(0, 512, (1, 12), generator=torch.Generator().manual_seed(1))
+    positions = torch.tensor([[0, 1, 2, 3, 4, 0, 1, 2, 0, 1, 2, 3]])
+    packed = dict(input_ids=ids, position_ids=positions, use_cache=False)
+    bounds = dict(cu_seq_lens_q=torch.tensor([0, 5, 8, 12]), cu_seq_lens_k=torch.tensor([0, 5, 8, 12]))
+    with torch.no_grad():
+        want = model(**packed).logits
+    monkeypatch.setattr(mb.model, "qk_norm_rope", plain_qk_norm_rope)
+    mb.model.install_attention(model)
+    with torch.no_grad():  # the model gives a mask for sequences told by their positions, with the bounds or without
+        for more in ({}, bounds):
+            torch.testing.assert_close(model(**packed, **more).logits, want, atol=1e-4, rtol=0)
+        with pytest.raises(NotImplementedError, match="packed"):
+            model(input_ids=ids, use_cache=False, **bounds)
+        model.set_attn_implementation("eager")
+        torch.testing.assert_close(model(**packed).logits, want, atol=1e-4, rtol=0)
+        with pytest.raises(NotImplementedError, match="output_attentions"):
+            model(**packed, output_attentions=True)
