@@ -134,6 +134,10 @@ def _attention_implementation(module):
 
 def _attention_forward(self, hidden_states, position_embeddings, attention_mask=None, past_key_values=None, **kwargs):
     """The attention's forward with norms and rotation in one pass between the projections and torch's attention."""
+    return _attention(self, qk_norm_rope, hidden_states, position_embeddings, attention_mask, past_key_values, **kwargs)
+
+
+def _attention(self, norm_rotate, hidden_states, position_embeddings, attention_mask, past_key_values=None, **kwargs):
     implementation = _attention_implementation(self)  # (it may have been changed since install_attention)
     if attention_mask is None and any(kwargs.get(n) is not None for n in ("cu_seq_lens_q", "cu_seq_lens_k")):
         raise NotImplementedError("packed sequences (cu_seq_lens) need an attention mask that separates them")
@@ -148,7 +152,7 @@ def _attention_forward(self, hidden_states, position_embeddings, attention_mask=
     if cos.shape[0] > 1:
         positions = torch.arange(batch * length, device=q.device).view(batch, length)
     cos, sin = (x.reshape(-1, 2 * half)[:, :half] for x in (cos, sin))
-    q, k = qk_norm_rope(q, k, self.q_norm.weight, self.k_norm.weight, cos, sin, positions=positions,
+    q, k = norm_rotate(q, k, self.q_norm.weight, self.k_norm.weight, cos, sin, positions=positions,
                         eps=self.q_norm.variance_epsilon)
     q, k, v = q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2)
     if past_key_values is not None:
@@ -165,12 +169,80 @@ def _attention_forward(self, hidden_states, position_embeddings, attention_mask=
 
 
 def _check_attention(name, module):
-    """Refuses an attention module that _attention_forward does not compute."""
+    """Refuses an attention module that _attention_forward does not compute: by what it says of itself, then by its own
+    forward on a few random tokens."""
     _attention_implementation(module)
     if getattr(module, "sliding_window", None) is not None:
         raise NotImplementedError(f"{name}: attention within a sliding window")
+    if not getattr(module, "is_causal", True):
+        raise NotImplementedError(f"{name}: attention that is not causal")
+    if not isinstance(getattr(module, "scaling", None), (int, float)) or not hasattr(module, "attention_dropout"):
+        raise NotImplementedError(f"{name}: the scale or the dropout of its attention is not known")
+    parts = ("q_proj", "k_proj", "v_proj", "o_proj", "q_norm", "k_norm")
+    other = [n for n, _ in module.named_parameters() if n.split(".")[0] not in parts]
+    if other:
+        raise NotImplementedError(f"{name}: attention with parameters of its own ({other[0]})")
+    for norm in (module.q_norm, module.k_norm):
+        if not hasattr(norm, "variance_epsilon") or tuple(getattr(norm, "weight", torch.empty(0)).shape) != (module.head_dim,):
+            raise NotImplementedError(f"{name}: norms over each head, with a weight of ({module.head_dim},), are expected")
     if module.q_norm.variance_epsilon != module.k_norm.variance_epsilon:
         raise NotImplementedError(f"{name}: norms of different epsilon")
+    if module.head_dim % 16 or module.head_dim > 256:
+        raise NotImplementedError(f"{name}: heads of {module.head_dim}: a multiple of 16 up to 256 is expected")
+    if getattr(module.forward, "__func__", None) is not _attention_forward:  # not patched before
+        _compare_attention(name, module)
+
+
+def _plain_norm_rotate(q, k, q_weight, k_weight, cos, sin, positions=None, eps=1e-6):
+    """qk_norm_rope in elementary operations (positions None), on any device."""
+    n = cos.shape[1]
+    cos, sin = (x.float()[:, None] for x in (cos, sin))
+
+    def heads(x, w):
+        y = x.float()
+        y = y * (y.square().mean(-1, keepdim=True) + eps).rsqrt() * w.float()
+        a, b = y[..., :n], y[..., n:2 * n]
+        return torch.cat([a * cos - b * sin, b * cos + a * sin, y[..., 2 * n:]], -1).to(x.dtype)
+
+    return heads(q, q_weight), heads(k, k_weight)
+
+
+@torch.no_grad()
+def _compare_attention(name, module, tokens=7):
+    """Raises unless the module's own forward does what _attention_forward would, on random tokens, angles and norm weights
+    (with its own, order and form of the norms may not show): within 5%, where bf16 rounds to 1% and a gate, a missing
+    rotation or another order of norm and rotation change the output altogether."""
+    weight = module.q_norm.weight
+    if any(p.is_meta for p in module.parameters()):
+        raise NotImplementedError(f"{name}: its weights are not loaded")
+    gen = torch.Generator().manual_seed(0)
+    like = dict(device=weight.device, dtype=module.q_proj.weight.dtype)
+    x = torch.randn((1, tokens, module.q_proj.weight.shape[1]), generator=gen).to(**like)
+    angle = (6.28 * torch.rand((1, tokens, module.head_dim // 2), generator=gen)).repeat(1, 1, 2)
+    angles = angle.cos().to(**like), angle.sin().to(**like)
+    mask = torch.full((1, 1, tokens, tokens), torch.finfo(x.dtype).min).triu(1).to(**like)
+    norms = {f"{n}.weight": (0.5 + torch.rand(weight.shape, generator=gen)).to(weight) for n in ("q_norm", "k_norm")}
+    modes = [(m, m.training) for m in module.modules()]
+    module.eval()
+    try:
+        call = dict(hidden_states=x, position_embeddings=angles, attention_mask=mask)
+        want = torch.func.functional_call(module, norms, kwargs=call)
+        before, module.forward = module.__dict__.get("forward"), types.MethodType(
+            lambda self, **kwargs: _attention(self, _plain_norm_rotate, **kwargs), module)
+        try:
+            got = torch.func.functional_call(module, norms, kwargs=call)
+        finally:
+            del module.forward
+            if before is not None:
+                module.forward = before
+    except (TypeError, ValueError, RuntimeError, AttributeError, IndexError, KeyError) as exc:
+        raise NotImplementedError(f"{name}: its forward does not run as a Qwen3 attention's ({exc})") from exc
+    finally:
+        for m, mode in modes:
+            m.training = mode
+    want, got = (y[0].float() if isinstance(y, tuple) else y.float() for y in (want, got))
+    if got.shape != want.shape or not bool((got - want).norm() <= 0.05 * want.norm()):
+        raise NotImplementedError(f"{name}: its forward is not a Qwen3 attention's")
 
 
 def install_attention(model) -> int:

@@ -165,3 +165,114 @@ def test_packed_sequences_and_attention_weights(monkeypatch):
         torch.testing.assert_close(model(**packed).logits, want, atol=1e-4, rtol=0)
         with pytest.raises(NotImplementedError, match="output_attentions"):
             model(**packed, output_attentions=True)
+
+
+def tiny(kind, **more):
+    """A small Transformers causal language model of one kind, its attention within heads of 32."""
+    import transformers
+
+    sizes = dict(vocab_size=128, hidden_size=128, intermediate_size=128, num_hidden_layers=2, num_attention_heads=4,
+                 num_key_value_heads=2, head_dim=32, max_position_embeddings=64, pad_token_id=0)
+    torch.manual_seed(0)
+    model = getattr(transformers, kind + "ForCausalLM")(getattr(transformers, kind + "Config")(**{**sizes, **more})).eval()
+    gen = torch.Generator().manual_seed(5)
+    for n, p in model.named_parameters():
+        if "_norm." in n:
+            p.data += 0.2 * torch.randn(p.shape, generator=gen)
+    return model
+
+
+MOE = dict(moe_intermediate_size=64, num_experts=4, num_experts_per_tok=2)
+
+
+@pytest.mark.parametrize("kind,more", [("Qwen3", {}), ("Qwen3Moe", MOE), ("Apertus", {}),
+                                       ("Glm4Moe", dict(use_qk_norm=True, n_routed_experts=4, num_experts_per_tok=2,
+                                                        moe_intermediate_size=64, partial_rotary_factor=0.5))],
+                         ids=lambda x: x if isinstance(x, str) else "")
+def test_attention_of_these_kinds_is_computed(monkeypatch, kind, more):
+    from transformers import StaticCache
+
+    model = tiny(kind, **more)
+    before = [p.clone() for p in model.parameters()]
+    ids = torch.randint(0, 128, (2, 9), generator=torch.Generator().manual_seed(1))
+    mask = torch.ones_like(ids)
+    mask[1, :4] = 0
+
+    def run():
+        with torch.no_grad():
+            first = model(input_ids=ids, use_cache=True)
+            static = StaticCache(config=model.config, max_cache_len=16)
+            return [first.logits, model(input_ids=ids, attention_mask=mask).logits[:, 4:],
+                    model(input_ids=ids[:, :1], past_key_values=first.past_key_values).logits,
+                    model(input_ids=ids[:, :5], past_key_values=static).logits,
+                    model(input_ids=ids[:, 5:6], past_key_values=static).logits]
+
+    want = run()
+    monkeypatch.setattr(mb.model, "qk_norm_rope", plain_qk_norm_rope)
+    assert mb.model.install_attention(model) == 2
+    assert mb.model.install_attention(model) == 2  # again
+    for g, w in zip(run(), want):
+        torch.testing.assert_close(g, w, atol=1e-4, rtol=0)
+    assert all(torch.equal(p, q) for p, q in zip(model.parameters(), before)) and not model.training
+
+
+@pytest.mark.parametrize("kind,more,why", [
+    ("Olmoe", MOE, "over each head"),  # norms over all heads
+    ("Afmoe", dict(MOE, layer_types=["full_attention"] * 2, num_dense_layers=1), "parameters of its own"),  # a gate
+    ("Doge", {}, "parameters of its own"),  # a mask it learns
+    ("Gemma3", None, "sliding window"),
+], ids=lambda x: x if isinstance(x, str) else "")
+def test_attention_of_other_kinds_is_refused(kind, more, why):
+    if more is None:
+        import transformers
+
+        model = transformers.Gemma3ForCausalLM(transformers.Gemma3TextConfig(
+            vocab_size=128, hidden_size=128, intermediate_size=128, num_hidden_layers=2, num_attention_heads=4,
+            num_key_value_heads=2, head_dim=32))
+    else:
+        model = tiny(kind, **more)
+    with pytest.raises(NotImplementedError, match=why):
+        mb.model.install_attention(model)
+
+
+@pytest.mark.parametrize("kind", ["order", "gate", "one plus the weight", "no rotation", "pairs", "not causal", "scale"])
+def test_attention_that_looks_alike_is_refused(kind):
+    """Modules with every attribute of a Qwen3 attention that compute something else."""
+    model = tiny("Qwen3")
+    attention = [a for _, a in mb.model.attention_modules(model)][1]
+    own = attention.forward
+
+    def forward(hidden_states, position_embeddings, attention_mask=None, past_key_values=None, **kwargs):
+        cos, sin = position_embeddings
+        batch, length = hidden_states.shape[:2]
+        q, k, v = (f(hidden_states).view(batch, length, -1, 32).transpose(1, 2)
+                   for f in (attention.q_proj, attention.k_proj, attention.v_proj))
+
+        def turn(x):
+            half = torch.cat([-x[..., 16:], x[..., :16]], -1)
+            if kind == "pairs":
+                half = torch.stack([-x[..., 1::2], x[..., ::2]], -1).flatten(-2)
+            return x * cos[:, None] + half * sin[:, None]
+
+        norms = attention.q_norm, attention.k_norm
+        if kind == "order":
+            q, k = (n(turn(x)) for n, x in zip(norms, (q, k)))
+        elif kind == "no rotation":
+            q, k = (n(x) for n, x in zip(norms, (q, k)))
+        elif kind == "one plus the weight":
+            q, k = (turn(n(x) / n.weight * (1 + n.weight)) for n, x in zip(norms, (q, k)))
+        else:
+            q, k = (turn(n(x)) for n, x in zip(norms, (q, k)))
+        out = torch.nn.functional.scaled_dot_product_attention(q, k, v, attn_mask=attention_mask, enable_gqa=True,
+                                                               scale=0.5 if kind == "scale" else None)
+        out = out.transpose(1, 2).reshape(batch, length, -1)
+        return attention.o_proj(out.sigmoid() * out if kind == "gate" else out), None
+
+    attention.forward = forward
+    if kind == "not causal":
+        attention.is_causal = False
+    with pytest.raises(NotImplementedError, match=kind if kind == "not causal" else "not a Qwen3"):
+        mb.model.install_attention(model)
+    assert attention.forward is forward
+    attention.forward, attention.is_causal = own, True
+    assert mb.model.install_attention(model) == 2
