@@ -262,17 +262,56 @@ def _routers(model):
     return [getattr(model.get_submodule(name.rpartition(".")[0]), "gate") for name, _ in experts_modules(model)]
 
 
+def _last_hidden(model, head, input_ids, attention_mask):
+    """The hidden states whose product with the head's weight is the model's logits.
+
+    The model runs its own forward, with the logits of the last position alone, and is watched: what it gives the head has
+    to be its decoder's last hidden states, and what it returns the head's output itself, or that divided by its
+    configuration's logits_scaling (Granite) or times its logit_scale (Cohere). The hidden states then take the scale, in
+    their own type: one rounding of theirs where the model's own path rounds every scaled logit. A model that does anything
+    else to its logits (a cap, an offset) is refused."""
+    decoder = model.get_decoder() if hasattr(model, "get_decoder") else model.model
+    states, products = [], []
+    hooks = [decoder.register_forward_hook(lambda m, args, out: states.append(out.last_hidden_state)),
+             head.register_forward_hook(lambda m, args, out: products.append(
+                 (args[0], out, out.clone() if out.is_inference() else out._version)), prepend=True)]
+    try:
+        out = model(input_ids=input_ids, attention_mask=attention_mask, use_cache=False, logits_to_keep=1, return_dict=True)
+    finally:
+        for h in hooks:
+            h.remove()
+    if len(states) != 1 or len(products) != 1:
+        raise NotImplementedError("a model that runs its decoder or its head more than once")
+    hidden, (given, product, mark) = states[0], products[0]
+    if (given.untyped_storage().data_ptr() != hidden.untyped_storage().data_ptr() or given.dtype != hidden.dtype
+            or given.shape[-1] != hidden.shape[-1]):
+        raise NotImplementedError("a model that changes its last hidden states before the head")
+    logits = out.logits
+    unchanged = torch.equal(product, mark) if torch.is_tensor(mark) else product._version == mark
+    if unchanged and logits.data_ptr() == product.data_ptr() and logits.dtype == product.dtype:
+        return hidden
+    config = model.config.get_text_config() if hasattr(model.config, "get_text_config") else model.config
+    divisor, factor = getattr(config, "logits_scaling", None), getattr(config, "logit_scale", None)
+    if unchanged and divisor is not None and torch.equal(logits, product / divisor):
+        return hidden / divisor
+    if unchanged and factor is not None and torch.equal(logits, product * factor):
+        return hidden * factor
+    raise NotImplementedError("a model that changes its logits after the head (a cap, for instance)")
+
+
 def training_loss(model, input_ids, labels, attention_mask=None, balance: float = 0.0, ignore_index: int = -100):
     """A fine-tuning step's loss of a Transformers causal language model, and the tokens of every expert: (loss, counts).
 
     The mean cross entropy of predicting labels (B, T) from the hidden states before each (labels are shifted here, as
-    Transformers does; `ignore_index` where there is none), from the head's weight without the logits; plus `balance`
+    Transformers does; `ignore_index` where there is none), from the head's weight without the logits but the last
+    position's, which show what the model does to them: a scale is applied, anything else refused. Plus `balance`
     times the routers' balance loss over the tokens that attention_mask (B, T) keeps, on the routers' own choices.
     counts: (layers, experts) int64, or None without balance (nothing is collected then)."""
-    base = model.get_decoder() if hasattr(model, "get_decoder") else model.model
     head = model.get_output_embeddings()
     if getattr(head, "bias", None) is not None:
         raise NotImplementedError("a head with a bias")
+    if type(head).forward is not torch.nn.Linear.forward:
+        raise NotImplementedError(f"a head that is a {type(head).__name__}: a linear layer is expected")
     seen, hooks = [], []
 
     def collect(router, args, out):
@@ -285,7 +324,7 @@ def training_loss(model, input_ids, labels, attention_mask=None, balance: float 
             raise NotImplementedError("the balance loss with gradient checkpointing: its routers run twice")
         hooks = [r.register_forward_hook(collect) for r in _routers(model)]
     try:
-        hidden = base(input_ids=input_ids, attention_mask=attention_mask, use_cache=False).last_hidden_state
+        hidden = _last_hidden(model, head, input_ids, attention_mask)
     finally:
         for h in hooks:
             h.remove()

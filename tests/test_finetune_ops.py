@@ -276,3 +276,80 @@ def test_attention_that_looks_alike_is_refused(kind):
     assert attention.forward is forward
     attention.forward, attention.is_causal = own, True
     assert mb.model.install_attention(model) == 2
+
+
+def plain_loss(hidden, weight, targets, ignore_index=-100, reduction="mean"):
+    logits = hidden.reshape(-1, hidden.shape[-1]).float() @ weight.float().t()
+    return torch.nn.functional.cross_entropy(logits, targets.reshape(-1), ignore_index=ignore_index, reduction=reduction)
+
+
+def trained_on():
+    ids = torch.randint(1, 128, (2, 11), generator=torch.Generator().manual_seed(2))
+    labels = ids.clone()
+    labels[:, :4] = -100
+    mask = torch.ones_like(ids)
+    mask[1, 8:] = 0
+    labels[mask == 0] = -100
+    return ids, labels, mask
+
+
+@pytest.mark.parametrize("kind,more", [("Qwen3Moe", MOE), ("GraniteMoe", dict(logits_scaling=6.0, num_local_experts=4)),
+                                       ("GraniteMoe", dict(logits_scaling=0.25, num_local_experts=4)),
+                                       ("Cohere", dict(logit_scale=0.0625)), ("Gemma2", dict(final_logit_softcapping=None)),
+                                       ("Llama", dict(tie_word_embeddings=True))],
+                         ids=lambda x: x if isinstance(x, str) else "")
+def test_the_training_loss_is_the_models_own(monkeypatch, kind, more):
+    """Models that scale their logits among them: the same loss and gradients in float32 as from the model's logits."""
+    monkeypatch.setattr(mb.model, "linear_cross_entropy", plain_loss)
+    model = tiny(kind, **more).train()
+    for m in model.modules():
+        if isinstance(m, torch.nn.Dropout):
+            m.p = 0.0
+    ids, labels, mask = trained_on()
+    want = model(input_ids=ids, labels=labels, attention_mask=mask).loss
+    params = [p for p in model.parameters() if p.requires_grad]
+    grads = torch.autograd.grad(want, params, allow_unused=True)
+    loss, counts = mb.model.training_loss(model, ids, labels, attention_mask=mask)
+    assert counts is None
+    torch.testing.assert_close(loss, want, atol=0, rtol=1e-5)
+    for got, w in zip(torch.autograd.grad(loss, params, allow_unused=True), grads):
+        assert (got is None) == (w is None)
+        if w is not None:
+            torch.testing.assert_close(got, w, atol=1e-5 * float(w.abs().max()), rtol=1e-3)
+    with torch.inference_mode():
+        again, _ = mb.model.training_loss(model, ids, labels, attention_mask=mask)
+    torch.testing.assert_close(again, loss.detach(), atol=0, rtol=1e-6)
+
+
+def test_models_that_do_more_to_their_logits_are_refused(monkeypatch):
+    monkeypatch.setattr(mb.model, "linear_cross_entropy", plain_loss)
+    ids, labels, mask = trained_on()
+
+    def refused(model, match):
+        with pytest.raises(NotImplementedError, match=match):
+            mb.model.training_loss(model, ids, labels, attention_mask=mask)
+        with torch.inference_mode(), pytest.raises(NotImplementedError, match=match):
+            mb.model.training_loss(model, ids, labels, attention_mask=mask)
+
+    refused(tiny("Gemma2", final_logit_softcapping=30.0), "after the head")
+    model = tiny("Qwen3")
+    hook = model.lm_head.register_forward_hook(lambda m, args, out: out + 1.0)
+    refused(model, "after the head")
+    hook.remove()
+    hook = model.lm_head.register_forward_hook(lambda m, args, out: out.mul_(2.0))
+    refused(model, "after the head")
+    hook.remove()
+    hook = model.lm_head.register_forward_pre_hook(lambda m, args: (args[0] * 0.5,))
+    refused(model, "before the head")
+    hook.remove()
+    mb.model.training_loss(model, ids, labels, attention_mask=mask)
+    assert not model.lm_head._forward_hooks and not model.model._forward_hooks
+
+    class Adapted(torch.nn.Linear):
+        def forward(self, x):
+            return super().forward(x) * 2.0
+
+    model.lm_head = Adapted(128, 128, bias=False)
+    refused(model, "linear layer")
+    model.lm_head = torch.nn.Linear(128, 128)
+    refused(model, "bias")

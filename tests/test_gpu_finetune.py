@@ -154,3 +154,27 @@ def test_decoding_behind_a_cache():
     mb.model.install_attention(model)
     for g, w in zip(run(), want):
         assert (g - w).norm() <= 3e-2 * w.norm()
+
+
+@pytest.mark.parametrize("scaling", [6.0, 0.25])
+def test_a_model_that_scales_its_logits(scaling):
+    """GraniteMoe divides its logits: the loss within bf16's rounding of the logits (which the model's own path has), the
+    gradients as the other whole-model comparisons."""
+    from transformers import GraniteMoeConfig, GraniteMoeForCausalLM
+
+    torch.manual_seed(0)
+    model = GraniteMoeForCausalLM(GraniteMoeConfig(
+        vocab_size=512, hidden_size=256, intermediate_size=128, num_hidden_layers=1, num_attention_heads=4,
+        num_key_value_heads=2, num_local_experts=4, num_experts_per_tok=2, logits_scaling=scaling)).to(DEV, torch.bfloat16)
+    for p in model.parameters():
+        p.requires_grad_(False)
+    model.model.norm.weight.requires_grad_()
+    model.model.layers[0].input_layernorm.weight.requires_grad_()
+    ids, labels, mask = batch(True)
+    out = model(input_ids=ids, labels=labels, attention_mask=mask)
+    out.loss.backward()
+    want_loss, want = out.loss.detach().float(), take(model)
+    loss, _ = mb.model.training_loss(model, ids, labels, attention_mask=mask)
+    loss.backward()
+    assert abs(loss.item() - want_loss.item()) <= 1e-2 * want_loss.item()
+    compare(take(model), want)
