@@ -258,8 +258,14 @@ def install_attention(model) -> int:
 
 
 def _routers(model):
-    """The routers beside the experts modules, in the layers' order."""
-    return [getattr(model.get_submodule(name.rpartition(".")[0]), "gate") for name, _ in experts_modules(model)]
+    """The routers beside the experts modules, in the layers' order: a `gate` whose weight alone gives the logits."""
+    routers = [getattr(model.get_submodule(name.rpartition(".")[0]), "gate", None) for name, _ in experts_modules(model)]
+    for r in routers:
+        if r is None or [n for n, _ in r.named_parameters()] != ["weight"]:
+            raise NotImplementedError("the balance loss: routers with one weight, as `gate` beside the experts, are expected")
+    if not routers:
+        raise NotImplementedError("the balance loss of a model without experts modules")
+    return routers
 
 
 def _last_hidden(model, head, input_ids, attention_mask):
@@ -315,7 +321,10 @@ def training_loss(model, input_ids, labels, attention_mask=None, balance: float 
     seen, hooks = [], []
 
     def collect(router, args, out):
-        # the router gives its probabilities and its choice; its logits are one small product more
+        # the router gives its probabilities, the weights and the choice; its logits are one small product more
+        if (not isinstance(out, tuple) or len(out) != 3 or not all(torch.is_tensor(x) and x.dim() == 2 for x in out)
+                or out[0].shape[1] != router.weight.shape[0] or out[2].dtype not in (torch.int64, torch.int32)):
+            raise NotImplementedError(f"the balance loss of a {type(router).__name__}: what it gives is not known")
         x = args[0]
         seen.append((torch.nn.functional.linear(x.reshape(-1, x.shape[-1]), router.weight), out[2]))
 
@@ -332,6 +341,8 @@ def training_loss(model, input_ids, labels, attention_mask=None, balance: float 
     loss = linear_cross_entropy(hidden, head.weight, targets, ignore_index=ignore_index)
     if not balance:
         return loss, None
+    if len(seen) != len(hooks):
+        raise NotImplementedError("the balance loss of routers that are not called as modules, once each")
     logits, index = zip(*seen)
     mask = None if attention_mask is None else attention_mask.reshape(-1)
     extra, counts = balance_loss(logits, index[0].shape[1], mask=mask, top_k_index=index)

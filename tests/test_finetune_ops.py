@@ -353,3 +353,50 @@ def test_models_that_do_more_to_their_logits_are_refused(monkeypatch):
     refused(model, "linear layer")
     model.lm_head = torch.nn.Linear(128, 128)
     refused(model, "bias")
+
+
+def plain_balance(logits, top_k, mask=None, top_k_index=None):
+    chosen = [torch.nn.functional.one_hot(i, x.shape[1]).sum(1) for x, i in zip(logits, top_k_index)]
+    live = torch.ones(len(logits[0]), dtype=torch.bool) if mask is None else mask != 0
+    n = len(logits) * int(live.sum())
+    f = sum(c[live].sum(0) for c in chosen).float() / n
+    m = sum(torch.softmax(x[live].float(), 1).sum(0) for x in logits) / n
+    counts = torch.stack([c[live].sum(0) for c in chosen])
+    return logits[0].shape[1] * (f * m).sum(), counts[0] if len(logits) == 1 else counts
+
+
+@pytest.mark.parametrize("kind", ["Qwen3Moe", "Mixtral", "Olmoe", "Qwen2Moe"])
+def test_the_balance_loss_of_these_routers(monkeypatch, kind):
+    monkeypatch.setattr(mb.model, "linear_cross_entropy", plain_loss)
+    monkeypatch.setattr(mb.model, "balance_loss", plain_balance)
+    model = tiny(kind, **dict(MOE, num_local_experts=4))
+    ids, labels, mask = trained_on()
+    probabilities = []
+    hooks = [r.register_forward_hook(lambda m, a, o: probabilities.append((o[0], o[2]))) for r in mb.model._routers(model)]
+    plain, _ = mb.model.training_loss(model, ids, labels, attention_mask=mask)
+    for h in hooks:
+        h.remove()
+    loss, counts = mb.model.training_loss(model, ids, labels, attention_mask=mask, balance=2.0)
+    want, counted = plain_balance([p.log() for p, _ in probabilities], 2, mask.reshape(-1), [i for _, i in probabilities])
+    torch.testing.assert_close(loss - plain, 2.0 * want, atol=1e-5, rtol=1e-5)
+    assert torch.equal(counts, counted) and not any(r._forward_hooks for r in mb.model._routers(model))
+
+
+@pytest.mark.parametrize("kind,more", [("Glm4Moe", dict(n_routed_experts=4, num_experts_per_tok=2, moe_intermediate_size=64)),
+                                       ("Ernie4_5_Moe", dict(moe_num_experts=4, moe_k=2, moe_intermediate_size=64,
+                                                             moe_layer_start_index=0)), ("GptOss", MOE), ("Qwen3", {}),
+                                       ("DeepseekV2", dict(n_routed_experts=4, num_experts_per_tok=2, n_group=1, topk_group=1,
+                                                           moe_intermediate_size=64, first_k_dense_replace=0, head_dim=16,
+                                                           qk_rope_head_dim=16, qk_nope_head_dim=16, v_head_dim=16,
+                                                           kv_lora_rank=32, q_lora_rank=None, num_key_value_heads=4))],
+                         ids=lambda x: x if isinstance(x, str) else "")
+def test_the_balance_loss_of_other_routers_is_refused(monkeypatch, kind, more):
+    """Corrected, biased or grouped choices, gates that are not called as modules, and models without experts."""
+    monkeypatch.setattr(mb.model, "linear_cross_entropy", plain_loss)
+    monkeypatch.setattr(mb.model, "balance_loss", plain_balance)
+    model = tiny(kind, **more)
+    ids, labels, mask = trained_on()
+    with pytest.raises(NotImplementedError, match="balance loss"):
+        mb.model.training_loss(model, ids, labels, attention_mask=mask, balance=0.1)
+    assert not any(m._forward_hooks for m in model.modules())
+    mb.model.training_loss(model, ids, labels, attention_mask=mask)
