@@ -141,6 +141,8 @@ def _attention(self, norm_rotate, hidden_states, position_embeddings, attention_
     implementation = _attention_implementation(self)  # (it may have been changed since install_attention)
     if attention_mask is None and any(kwargs.get(n) is not None for n in ("cu_seq_lens_q", "cu_seq_lens_k")):
         raise NotImplementedError("packed sequences (cu_seq_lens) need an attention mask that separates them")
+    if kwargs.get("is_causal") is False:
+        raise NotImplementedError("attention that is not causal (is_causal)")
     if implementation == "eager" and (kwargs.get("output_attentions") or getattr(self.config, "output_attentions", False)):
         raise NotImplementedError("attention weights (output_attentions) are not computed")
     batch, length = hidden_states.shape[:2]

@@ -400,3 +400,14 @@ def test_the_balance_loss_of_other_routers_is_refused(monkeypatch, kind, more):
         mb.model.training_loss(model, ids, labels, attention_mask=mask, balance=0.1)
     assert not any(m._forward_hooks for m in model.modules())
     mb.model.training_loss(model, ids, labels, attention_mask=mask)
+
+
+def test_a_call_that_is_not_causal_is_refused(monkeypatch):
+    monkeypatch.setattr(mb.model, "qk_norm_rope", plain_qk_norm_rope)
+    model = tiny("Qwen3")
+    mb.model.install_attention(model)
+    attention = next(mb.model.attention_modules(model))[1]
+    x, angles = torch.randn((1, 4, 128)), (torch.ones((1, 4, 32)), torch.zeros((1, 4, 32)))
+    with pytest.raises(NotImplementedError, match="not causal"):
+        attention(x, position_embeddings=angles, attention_mask=None, is_causal=False)
+    attention(x, position_embeddings=angles, attention_mask=None, is_causal=True)
