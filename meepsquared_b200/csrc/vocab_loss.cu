@@ -33,6 +33,8 @@
 // The tensor cores cut every step's sum off toward zero. Over the 256 steps of a logit of 4,096 products that made the
 // mean loss 1.1e-6 of itself too small; so beyond 2,048 products a logit's sum is taken from tensor memory every 2,048
 // and joined in the epilogue's registers (DEEP), with ordinary float32 additions.
+#include <atomic>
+
 #include "common.cuh"
 #include "host.hpp"
 
@@ -978,10 +980,11 @@ template <int MODE, bool REDO, bool DEEP, bool SOLO>
 static int launch_product(const CUtensorMap& a, const CUtensorMap& a32, const CUtensorMap& b, const CUtensorMap& out,
                           const Params& p, int pairs, cudaStream_t s, bool after) {
   auto kern = vocab_product<MODE, REDO, DEEP, SOLO>;
-  static uint64_t configured = 0;  // per device: a function's attributes are set on the current one
+  // per device (a function's attributes are set on the current one); threads may call at once, each then configures
+  static std::atomic<uint64_t> configured{0};
   int device = 0;
   if (cudaGetDevice(&device) != cudaSuccess) return cudaGetLastError(), MEEP2B_ERR_LAUNCH;
-  if (device >= 64 || !((configured >> device) & 1)) {
+  if (device >= 64 || !((configured.load(std::memory_order_acquire) >> device) & 1)) {
     // DEEP's register split adds up to 168 a thread at launch: with fewer the increase would never be granted
     cudaFuncAttributes attr;
     if (cudaFuncGetAttributes(&attr, kern) != cudaSuccess || (DEEP && attr.numRegs != 168) ||
@@ -989,7 +992,7 @@ static int launch_product(const CUtensorMap& a, const CUtensorMap& a32, const CU
       cudaGetLastError();
       return MEEP2B_ERR_LAUNCH;
     }
-    if (device < 64) configured |= uint64_t(1) << device;
+    if (device < 64) configured.fetch_or(uint64_t(1) << device, std::memory_order_release);
   }
   return launch_in(SOLO ? 1 : 2, after, kern, 2u * pairs, Epi<MODE, DEEP>::THREADS, SMEM_BYTES, s, a, a32, b, out, p);
 }

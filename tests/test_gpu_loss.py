@@ -440,3 +440,36 @@ def test_forward_mode_derivatives_are_refused(which):
         torch.func.jvp(lambda x: call(*[x if i == which else y for i, y in enumerate(given)]), (given[which],),
                        (torch.ones_like(given[which]),))
     call(*given)  # and nothing is left behind
+
+
+def test_the_first_calls_of_a_process_from_several_threads():
+    """Every kernel is set up at its first launch, here by threads that come at once (in a process of its own)."""
+    import os
+    import subprocess
+    import sys
+
+    code = """
+import threading, torch
+import meepsquared_b200 as mb
+gen = torch.Generator().manual_seed(0)
+h, w = (torch.randn(s, generator=gen).to("cuda", torch.bfloat16) for s in ((300, 72), (600, 72)))
+t = torch.randint(0, 600, (300,), generator=gen).cuda()
+start, results = threading.Barrier(6), [None] * 6
+def one(i):
+    a, b = h.detach().requires_grad_(), w.detach().requires_grad_(i % 2 == 1)
+    with torch.cuda.stream(torch.cuda.Stream()):
+        start.wait()
+        loss = mb.linear_cross_entropy(a, b, t)
+        loss.backward()
+        torch.cuda.current_stream().synchronize()
+    results[i] = loss.detach(), a.grad
+torch.cuda.synchronize()
+threads = [threading.Thread(target=one, args=(i,)) for i in range(6)]
+[x.start() for x in threads], [x.join() for x in threads]
+for i in range(2, 6):
+    assert torch.equal(results[i][0], results[i % 2][0]) and torch.equal(results[i][1], results[i % 2][1])
+print("alike")
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(mb.__file__)))  # of the package
+    done = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=240)
+    assert done.returncode == 0 and "alike" in done.stdout, done.stderr[-2000:]
