@@ -166,12 +166,17 @@ def native():
     """The compiled autograd nodes of the fine-tuning operators (csrc/native.cpp), which call libmeep2b."""
     global _native
     if _native is None:
+        from . import build
+
         load()
         try:
             from . import _native as module
         except ImportError as exc:
             raise RuntimeError(f"_native.so is not built or does not load ({exc}); run `python -m "
                                "meepsquared_b200.build`") from exc
+        if module.built_for != build.native_tag():
+            raise RuntimeError(f"_native.so was {module.built_for}, not {build.native_tag()}; run `python -m "
+                               "meepsquared_b200.build`")
         _native = module
     return _native
 

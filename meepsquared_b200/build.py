@@ -48,9 +48,20 @@ def build(verbose: bool = False, force: bool = False) -> str:
     return LIB
 
 
+def native_tag() -> str:
+    """What the autograd nodes' layout depends on (torch, its C++ ABI, the interpreter's): _native.so holds it."""
+    import torch
+
+    return f"built for torch {torch.__version__}, ABI {int(torch._C._GLIBCXX_USE_CXX11_ABI)}, " \
+           f"{sysconfig.get_config_var('EXT_SUFFIX')}"
+
+
 def native_stale() -> bool:
     if not os.path.exists(NATIVE):
         return True
+    with open(NATIVE, "rb") as f:
+        if native_tag().encode() not in f.read():
+            return True
     t = os.path.getmtime(NATIVE)
     return any(os.path.getmtime(d) > t for d in (NATIVE_SOURCE, os.path.join(HERE, "..", "include", "meep2b.h")))
 
@@ -64,6 +75,7 @@ def build_native(verbose: bool = False) -> str:
     includes = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
                 sysconfig.get_paths()["include"], os.path.join(cuda, "include")]
     cmd = [cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-DTORCH_EXTENSION_NAME=_native",
+           f'-DMEEP2B_NATIVE_TAG="{native_tag()}"',
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *[f"-I{d}" for d in includes], NATIVE_SOURCE,
            "-o", NATIVE + ".tmp", f"-L{HERE}", "-l:" + os.path.basename(LIB), "-L" + os.path.join(root, "lib"), "-lc10",
            "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]

@@ -410,6 +410,7 @@ Tensor linear_cross_entropy(const Tensor& hidden, const Tensor& weight, const Te
 }  // namespace
 
 PYBIND11_MODULE(_native, m) {
+  m.attr("built_for") = MEEP2B_NATIVE_TAG;
   // without the interpreter's lock, as ctypes calls: a full launch queue blocks no other thread
   m.def("qk_norm_rope", &qk_norm_rope, py::call_guard<py::gil_scoped_release>());
   m.def("balance_loss", &balance_loss, py::call_guard<py::gil_scoped_release>());

@@ -411,3 +411,17 @@ def test_a_call_that_is_not_causal_is_refused(monkeypatch):
     with pytest.raises(NotImplementedError, match="not causal"):
         attention(x, position_embeddings=angles, attention_mask=None, is_causal=False)
     attention(x, position_embeddings=angles, attention_mask=None, is_causal=True)
+
+
+def test_nodes_built_for_another_torch_are_rebuilt_and_not_loaded(monkeypatch):
+    """The compiled autograd nodes hold torch's class layouts: a file that another torch, ABI or interpreter built is stale,
+    whatever its time."""
+    build.build()
+    assert not build.native_stale()
+    tag = build.native_tag()
+    assert torch.__version__ in tag
+    monkeypatch.setattr(build, "native_tag", lambda: tag.replace(torch.__version__, "9.9.9"))
+    assert build.native_stale()
+    monkeypatch.setattr(_lib, "_native", None)
+    with pytest.raises(RuntimeError, match="was built for torch"):
+        _lib.native()
