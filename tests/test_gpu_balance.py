@@ -310,3 +310,29 @@ def test_forward_mode_derivatives_are_refused(which):
         torch.func.jvp(lambda x: call(*[x if i == which else y for i, y in enumerate(inputs)]), (inputs[which],),
                        (torch.ones_like(inputs[which]),))
     call(*inputs)  # and nothing is left behind
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_captured_in_a_graph(dtype):
+    xs = [x.requires_grad_() for x in make(3, 200, 64, dtype)]
+    mask = torch.arange(200, device=DEV) % 7 != 0
+
+    def step():
+        loss, counts = mb.balance_loss(xs, 6, mask=mask)
+        return loss.detach(), counts, *torch.autograd.grad(loss, xs)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for seed in (5, 6):
+        with torch.no_grad():
+            for x, new in zip(xs, make(3, 200, 64, dtype, seed)):
+                x.copy_(new)
+        graph.replay()
+        for a, b in zip(out, step()):
+            assert torch.equal(a, b)

@@ -358,3 +358,30 @@ def test_forward_mode_derivatives_are_refused(which):
         torch.func.jvp(lambda x: call(*[x if i == which else y for i, y in enumerate(inputs)]), (inputs[which],),
                        (torch.ones_like(inputs[which]),))
     call(*inputs)  # and nothing is left behind
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_captured_in_a_graph(dtype):
+    q, k, wq, wk, dq, dk = make(2, 30, 4, 2, 64, dtype)
+    leaves = [x.detach().requires_grad_() for x in (q, k, wq, wk)]
+    cos, sin = angles(30, 32)
+
+    def step():
+        out = mb.qk_norm_rope(*leaves, cos, sin)
+        return *(x.detach() for x in out), *torch.autograd.grad(out, leaves, [dq, dk])
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for seed in (5, 6):
+        with torch.no_grad():
+            for x, new in zip(leaves, make(2, 30, 4, 2, 64, dtype, seed)):
+                x.copy_(new)
+        graph.replay()
+        for a, b in zip(out, step()):
+            assert torch.equal(a, b)
