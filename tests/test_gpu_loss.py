@@ -494,3 +494,19 @@ def test_the_mean_loss_is_not_cut_off(hidden):
         want += float((torch.logsumexp(z, 1) - z.gather(1, b[:, None])[:, 0]).sum())
     got = float(mb.linear_cross_entropy(h, w, t).double())
     assert abs(got * tokens - want) <= 7e-7 * want
+
+
+@pytest.mark.parametrize("tokens,hidden,vocab", [(16384, 512, 600), (300, 2048, 600), (70000, 2048, 300)])
+def test_what_a_frozen_heads_graph_holds(tokens, hidden, vocab):
+    """Between forward and backward: the gradient's planes, 512 MB or one of tokens (up to a multiple of 256) x hidden in
+    float32 where that is more, and 40 bytes or so a token."""
+    h = torch.zeros((tokens, hidden), dtype=torch.bfloat16, device=DEV).requires_grad_()
+    w = torch.zeros((vocab, hidden), dtype=torch.bfloat16, device=DEV)
+    t = torch.zeros((tokens,), dtype=torch.int64, device=DEV)
+    before = torch.cuda.memory_allocated()
+    loss = mb.linear_cross_entropy(h, w, t)
+    held = torch.cuda.memory_allocated() - before
+    assert held <= max(1 << 29, (tokens + 255) // 256 * 256 * hidden * 4) + 64 * tokens + (1 << 16)
+    loss.backward()
+    del loss
+    assert torch.cuda.memory_allocated() - before <= tokens * hidden * 2 + (1 << 16)
