@@ -17,8 +17,10 @@
 // and then between lanes: about 60 instructions a token at 128 experts, where top_k rounds of a maximum over all keys
 // took 140. More than 8, or float32 logits (64-bit keys), take the rounds.
 //
-// 24 layers of 16,384 x 128 bf16: forward 75 us (112 instructions a token; the integer pipe's minima and maxima bound
-// it, 1.3 TB/s), backward 43 us (4.7 TB/s); the rounds took 174 us forward.
+// 24 layers of 16,384 x 128 (8 chosen), kernels alone: bf16 logits, own choice 78 us (1.3 TB/s), choice given 47, backward
+// 44 (4.6 TB/s); float32 logits 227, 61 and 66. The top_k rounds took 174 us in bf16. What bounds the forward pass is
+// latency: at 128 registers a thread there are 3.5 warps a scheduler and 0.59 instructions issued a cycle; the integer
+// pipe (minima and maxima) is the busiest, 64% in bf16 and 79% in float32, whose 64-bit keys also spill.
 //
 // The probabilities' sums stay in float32 registers over up to 256 of a group's tokens (equal probabilities, one after
 // another, would be off by 9e-5 of their sum after 7,000) and are joined per CTA in 64 bits; the CTAs' sums are added as

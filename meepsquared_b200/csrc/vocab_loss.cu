@@ -25,14 +25,22 @@
 //   kAcc      dh's product: piece x W, float32, stored by the first piece and added (TMA reduction) by the others
 //   kWeight   dW's product: piece^T x h, bf16
 //
-// Bound by the tensor pipe where hidden and rows are large (82-88% active alone; 16,384 tokens x 131,072 at hidden
-// 2048, loss and dh: 13.2-14.2 ms, 1.23-1.34 PFLOP/s at the power cap), by the epilogue's exponentials below hidden
-// 512 or so (8,192 tokens x 50,000 at hidden 64: 174 us), and by reading the head for few rows (37 tokens x 131,072:
-// 104 us for 537 MB).
+// Bound by the tensor pipe where hidden and rows are large (alone, at 2,048 tokens x 32,768: 84-88% active for the
+// products over the logits, 82% for dW's and 77% for dh's, whose 64 units leave some of 74 pairs idle; 16,384 tokens x
+// 131,072 at hidden 2048, loss and dh: 13.2-14.3 ms, 1.23-1.34 PFLOP/s at the power cap), by the epilogue's exponentials
+// below hidden 512 or so (8,192 tokens x 50,000 at hidden 64: 174 us), and by reading the head for few rows (37 tokens x
+// 131,072: 118 us for 537 MB, the L2 cache flushed before each call).
+//
+// q and g (p - [v = y]) are rounded to bf16 because both operands of the second products have one type, and the head's
+// is bf16. dh hardly notices (2e-4 of its norm, against 1.66e-3 for its own rounding): its largest term by far, the
+// target's, is kept apart in float32. dW's terms are all rounded before they are summed over the tokens: 1.9e-3 of its
+// norm instead of 1.6e-3, and 1.5e-4 too long along itself (targets of little probability, whose 1 - p rounds to 1).
 //
 // The tensor cores cut every step's sum off toward zero. Over the 256 steps of a logit of 4,096 products that made the
 // mean loss 1.1e-6 of itself too small; so beyond 2,048 products a logit's sum is taken from tensor memory every 2,048
-// and joined in the epilogue's registers (DEEP), with ordinary float32 additions.
+// and joined in the epilogue's registers (DEEP), with ordinary float32 additions (the loss is then 5e-7 too small at 4,096
+// products, 2.5e-7 at 2,048). dh's product sums a whole piece of the vocabulary in tensor memory: measured along itself
+// it is 2e-6 (4,093 tokens x 131,072) and 1.4e-5 (trained head, 32,003 at hidden 4096) too short, far below its rounding.
 #include <atomic>
 
 #include "common.cuh"
@@ -48,9 +56,14 @@ constexpr int RING_BYTES = 192 * 1024;
 
 // A unit is 256 rows on a CTA pair, each CTA with its 128 rows and half of the 256 columns; or (SOLO) 128 rows on one
 // CTA with all 256 columns, which loads half as much again for each product. Single CTAs are taken where a pair's
-// last 128 rows would be empty and are a good part of all (few_rows: an odd number of 128-row tiles, up to five).
-// Loss alone at hidden 2048, vocabulary 131,072, pairs against single CTAs: 37 tokens 117 and 104 us, 200 tokens 127
-// and 140, 300 tokens 217 and 180, 512 tokens 204 and 219.
+// last 128 rows would be empty and are a good part of all (few_rows: an odd number of 128-row tiles, up to five; of all
+// tokens, since the host does not know how many have a target). Loss alone at hidden 2048, the L2 cache flushed, us with
+// single CTAs / with pairs, by the vocabulary:
+//            37 tokens   300 tokens   513-640 tokens
+//    16,384   38 / 34      49 / 45       60 / 54
+//    32,768   46 / 50      66 / 69       87 / 85
+//   131,072  118 / 120    176 / 197   255-290 / 270-320
+// and with the gradient at 131,072: 223 / 236, 383 / 427, 565 / 575. Pairs win where the vocabulary is short of units.
 inline bool few_rows(int64_t tokens) {
   const int64_t tiles = (tokens + 127) / 128;
   return tiles % 2 == 1 && tiles <= 5;
