@@ -218,12 +218,14 @@ def _compare_attention(name, module, tokens=7):
     if any(p.is_meta for p in module.parameters()):
         raise NotImplementedError(f"{name}: its weights are not loaded")
     gen = torch.Generator().manual_seed(0)
-    like = dict(device=weight.device, dtype=module.q_proj.weight.dtype)
-    x = torch.randn((1, tokens, module.q_proj.weight.shape[1]), generator=gen).to(**like)
+    kind = module.q_proj.weight.dtype  # what a quantised projection stores is not what it takes
+    like = dict(device=weight.device, dtype=kind if kind in (torch.float32, torch.bfloat16, torch.float16) else weight.dtype)
+    width = getattr(module.q_proj, "in_features", module.q_proj.weight.shape[-1])
+    x = torch.randn((1, tokens, width), generator=gen).to(**like)
     angle = (6.28 * torch.rand((1, tokens, module.head_dim // 2), generator=gen)).repeat(1, 1, 2)
     angles = angle.cos().to(**like), angle.sin().to(**like)
     mask = torch.full((1, 1, tokens, tokens), torch.finfo(x.dtype).min).triu(1).to(**like)
-    norms = {f"{n}.weight": (0.5 + torch.rand(weight.shape, generator=gen)).to(weight) for n in ("q_norm", "k_norm")}
+    norms = {f"{n}.weight": (0.5 + torch.rand(weight.shape, generator=gen)).to(**like) for n in ("q_norm", "k_norm")}
     modes = [(m, m.training) for m in module.modules()]
     module.eval()
     try:

@@ -425,3 +425,31 @@ def test_nodes_built_for_another_torch_are_rebuilt_and_not_loaded(monkeypatch):
     monkeypatch.setattr(_lib, "_native", None)
     with pytest.raises(RuntimeError, match="was built for torch"):
         _lib.native()
+
+
+class Packed(torch.nn.Module):
+    """A projection whose weight is stored in another form than it computes in, as quantised ones are."""
+
+    def __init__(self, linear):
+        super().__init__()
+        self.in_features, self.out_features = linear.in_features, linear.out_features
+        self.held = [linear]
+        self.weight = torch.nn.Parameter(torch.zeros((linear.weight.numel() // 2, 1), dtype=torch.uint8), requires_grad=False)
+
+    def forward(self, x):
+        return torch.nn.functional.linear(x.float(), self.held[0].weight).to(x.dtype)
+
+
+@pytest.mark.parametrize("norms", [torch.float32, torch.bfloat16])
+def test_attention_with_quantised_projections_or_wider_norms_is_taken(norms):
+    """Packed projections (QLoRA), and norms kept in float32 beside projections in bf16."""
+    model = tiny("Qwen3")
+    for _, a in mb.model.attention_modules(model):
+        for n in ("q_proj", "k_proj", "v_proj", "o_proj"):
+            setattr(a, n, Packed(getattr(a, n)))
+        a.q_norm.to(norms), a.k_norm.to(norms)
+    assert mb.model.install_attention(model) == 2
+    model = tiny("Qwen3").to(torch.bfloat16)
+    for _, a in mb.model.attention_modules(model):
+        a.q_norm.to(norms), a.k_norm.to(norms)
+    assert mb.model.install_attention(model) == 2
