@@ -24,6 +24,7 @@ module's stacks: a ``gate_up_proj`` means gated, no ``*_bias`` means unbiased, a
 hidden) is not transposed.
 """
 
+import inspect
 import math
 import types
 
@@ -275,7 +276,8 @@ def _routers(model):
 def _last_hidden(model, head, input_ids, attention_mask):
     """The hidden states whose product with the head's weight is the model's logits.
 
-    The model runs its own forward, with the logits of the last position alone, and is watched: what it gives the head has
+    The model runs its own forward, with the logits of the last position alone (all of them where it knows no
+    logits_to_keep), and is watched: what it gives the head has
     to be its decoder's last hidden states, and what it returns the head's output itself, or that divided by its
     configuration's logits_scaling (Granite) or times its logit_scale (Cohere). The hidden states then take the scale, in
     their own type: one rounding of theirs where the model's own path rounds every scaled logit. A model that does anything
@@ -285,8 +287,10 @@ def _last_hidden(model, head, input_ids, attention_mask):
     hooks = [decoder.register_forward_hook(lambda m, args, out: states.append(out.last_hidden_state)),
              head.register_forward_hook(lambda m, args, out: products.append(
                  (args[0], out, out.clone() if out.is_inference() else out._version)), prepend=True)]
+    takes = inspect.signature(model.forward).parameters.values()
+    one = {"logits_to_keep": 1} if any(p.name == "logits_to_keep" or p.kind is p.VAR_KEYWORD for p in takes) else {}
     try:
-        out = model(input_ids=input_ids, attention_mask=attention_mask, use_cache=False, logits_to_keep=1, return_dict=True)
+        out = model(input_ids=input_ids, attention_mask=attention_mask, use_cache=False, return_dict=True, **one)
     finally:
         for h in hooks:
             h.remove()
@@ -297,15 +301,18 @@ def _last_hidden(model, head, input_ids, attention_mask):
             or given.shape[-1] != hidden.shape[-1]):
         raise NotImplementedError("a model that changes its last hidden states before the head")
     logits = out.logits
-    unchanged = torch.equal(product, mark) if torch.is_tensor(mark) else product._version == mark
-    if unchanged and logits.data_ptr() == product.data_ptr() and logits.dtype == product.dtype:
-        return hidden
-    config = model.config.get_text_config() if hasattr(model.config, "get_text_config") else model.config
-    divisor, factor = getattr(config, "logits_scaling", None), getattr(config, "logit_scale", None)
-    if unchanged and divisor is not None and torch.equal(logits, product / divisor):
-        return hidden / divisor
-    if unchanged and factor is not None and torch.equal(logits, product * factor):
-        return hidden * factor
+    if (torch.equal(product, mark) if torch.is_tensor(mark) else product._version == mark):  # not changed in place
+        if logits.dtype == product.dtype and logits.data_ptr() == product.data_ptr():
+            return hidden
+        product = product.to(logits.dtype)
+        config = model.config.get_text_config() if hasattr(model.config, "get_text_config") else model.config
+        divisor, factor = getattr(config, "logits_scaling", None), getattr(config, "logit_scale", None)
+        if divisor is not None and torch.equal(logits, product / divisor):
+            return hidden / divisor
+        if factor is not None and torch.equal(logits, product * factor):
+            return hidden * factor
+        if logits.dtype != hidden.dtype and torch.equal(logits, product):  # widened, as older Transformers do
+            return hidden
     raise NotImplementedError("a model that changes its logits after the head (a cap, for instance)")
 
 
@@ -317,6 +324,7 @@ def training_loss(model, input_ids, labels, attention_mask=None, balance: float 
     position's, which show what the model does to them: a scale is applied, anything else refused. Plus `balance`
     times the routers' balance loss over the tokens that attention_mask (B, T) keeps, on the routers' own choices.
     counts: (layers, experts) int64, or None without balance (nothing is collected then)."""
+    model = getattr(model, "_orig_mod", model)  # of a compiled model: its modules are watched
     head = model.get_output_embeddings()
     if getattr(head, "bias", None) is not None:
         raise NotImplementedError("a head with a bias")

@@ -453,3 +453,43 @@ def test_attention_with_quantised_projections_or_wider_norms_is_taken(norms):
     for _, a in mb.model.attention_modules(model):
         a.q_norm.to(norms), a.k_norm.to(norms)
     assert mb.model.install_attention(model) == 2
+
+
+@pytest.mark.parametrize("form", ["own", "float", "no logits_to_keep", "compiled", "float and capped"])
+def test_the_training_loss_of_other_forms_of_models(monkeypatch, form):
+    """Models that widen their logits (older Transformers), that know no logits_to_keep, that were compiled; in bf16."""
+    import types
+
+    from transformers import Qwen3ForCausalLM
+    from transformers.modeling_outputs import CausalLMOutputWithPast
+
+    monkeypatch.setattr(mb.model, "linear_cross_entropy", plain_loss)
+
+    class Widening(Qwen3ForCausalLM):
+        def forward(self, logits_to_keep=0, **kwargs):
+            out = super().forward(logits_to_keep=logits_to_keep, **kwargs)
+            logits = out.logits.float()
+            return CausalLMOutputWithPast(logits=20 * torch.tanh(logits / 20) if "capped" in form else logits)
+
+    class Plain(Qwen3ForCausalLM):
+        def forward(self, input_ids=None, attention_mask=None, use_cache=None, return_dict=None):
+            hidden = self.model(input_ids=input_ids, attention_mask=attention_mask, use_cache=use_cache)[0]
+            return types.SimpleNamespace(logits=self.lm_head(hidden))
+
+    model = tiny("Qwen3").to(torch.bfloat16)
+    ids, labels, mask = trained_on()
+    with torch.no_grad():
+        hidden = model.model(input_ids=ids, attention_mask=mask, use_cache=False).last_hidden_state
+        want = plain_loss(hidden[:, :-1], model.lm_head.weight, labels[:, 1:])
+    if form.startswith("float"):
+        model.__class__ = Widening
+    elif form == "no logits_to_keep":
+        model.__class__ = Plain
+    elif form == "compiled":
+        model = torch.compile(model, backend="eager")
+    if form == "float and capped":
+        with pytest.raises(NotImplementedError, match="after the head"):
+            mb.model.training_loss(model, ids, labels, attention_mask=mask)
+        return
+    loss, _ = mb.model.training_loss(model, ids, labels, attention_mask=mask)
+    torch.testing.assert_close(loss.detach(), want, atol=0, rtol=1e-6)
