@@ -34,7 +34,7 @@
 // q and g (p - [v = y]) are rounded to bf16 because both operands of the second products have one type, and the head's
 // is bf16. dh hardly notices (2e-4 of its norm, against 1.66e-3 for its own rounding): its largest term by far, the
 // target's, is kept apart in float32. dW's terms are all rounded before they are summed over the tokens: 1.9e-3 of its
-// norm instead of 1.6e-3, and 1.5e-4 too long along itself (targets of little probability, whose 1 - p rounds to 1).
+// norm instead of 1.6e-3 (up to 2.4e-3 where few tokens share a target), and 1.5e-4 too long along itself (targets of little probability, whose 1 - p rounds to 1).
 //
 // The tensor cores cut every step's sum off toward zero. Over the 256 steps of a logit of 4,096 products that made the
 // mean loss 1.1e-6 of itself too small; so beyond 2,048 products a logit's sum is taken from tensor memory every 2,048
